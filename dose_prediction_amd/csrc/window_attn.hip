@@ -1,0 +1,904 @@
+// Attention over a sliding window whose first tokens stay visible, forward and backward: the form of the ViT's attention for token rows
+// that are too long for the full one (attention.hip: finer patches, larger crops than the 512 .. 1152 tokens of dose_pyfer.py:55-67).
+//
+//   key j is seen by the query at position p  iff  p < n, j < n, j <= p + right and (j >= p - left or j < sinks)   (n: valid tokens)
+//   O = softmax(scale Q K^T) V over the seen keys; a query that sees nothing, or lies outside [0, n), gives 0.
+//   backward, from lse = log2 sum exp2(scale log2e s):  P = exp2(c s - lse), dV = P^T dO, dS = P (dO V^T - delta) scale, dQ = dS K,
+//   dK = dS^T Q with delta = rowsum(dO O).  Two passes without atomics (dQ by query rows, dK / dV by key rows): 14 d flop per pair
+//   instead of 10, and the same bits every time.
+//
+// Rows: the query heads that share a key head stand beside each other, row r = (token r / group, head r % group), so that one staged key
+// tile serves all of them and a single token with a group of heads is one tile.
+// Matrix tiles are 32 x 32 (k = 16).  The score tile is computed transposed (streamed rows x owned columns): a lane then holds one owned
+// row's scores, and the accumulator registers are, pair by pair of 8-row groups, the B operand of the second product; its A operand is
+// the streamed tile read k-major from LDS (ds_read_b64_tr_b16).  Running maximum and sum are one register per lane, fp32.
+#include "common.h"
+
+#define STREAM ((hipStream_t)stream)
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int FAR = 1 << 30;            // no limit on this side of the window
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ v16f mma32(const Frag8<bf16_t>& a, const Frag8<bf16_t>& b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a.u), __builtin_bit_cast(v8bf, b.u), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mma32(const Frag8<f16_t>& a, const Frag8<f16_t>& b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a.u), __builtin_bit_cast(v8h, b.u), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mma32(const Frag8<float>& a, const Frag8<float>& b, v16f c) {      // exact fp32 chain, same k slots
+#pragma unroll
+  for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ v16f zero16() { v16f z; for (int i = 0; i < 16; i++) z[i] = 0.f; return z; }
+
+template <typename T> __device__ __forceinline__ Frag8<T> ldg8(const T* p) { Frag8<T> f; f.u = *(const v4u*)p; return f; }
+template <> __device__ __forceinline__ Frag8<float> ldg8<float>(const float* p) { return frag_ld_lds(p); }
+__device__ __forceinline__ Frag8<bf16_t> pack8(const float* p, bf16_t) {
+  Frag8<bf16_t> f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) f.u[i] = (unsigned)f2bf(p[2 * i]) | ((unsigned)f2bf(p[2 * i + 1]) << 16);
+  return f;
+}
+__device__ __forceinline__ Frag8<f16_t> pack8(const float* p, f16_t) {
+  Frag8<f16_t> f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) f.u[i] = (unsigned)__builtin_bit_cast(unsigned short, (f16_t)p[2 * i]) | ((unsigned)__builtin_bit_cast(unsigned short, (f16_t)p[2 * i + 1]) << 16);
+  return f;
+}
+__device__ __forceinline__ Frag8<float> pack8(const float* p, float) {
+  Frag8<float> f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) f.v[i] = p[i];
+  return f;
+}
+template <typename T> __device__ __forceinline__ float elem(const Frag8<T>& f, int i) {
+  const unsigned short h = (unsigned short)(f.u[i >> 1] >> (16 * (i & 1)));
+  return ld_f((const T*)&h);
+}
+template <> __device__ __forceinline__ float elem<float>(const Frag8<float>& f, int i) { return f.v[i]; }
+__device__ __forceinline__ void st4(float* p, const float* v) { *(v4f*)p = (v4f){v[0], v[1], v[2], v[3]}; }
+__device__ __forceinline__ void st4(bf16_t* p, const float* v) {
+  *(uint2*)p = make_uint2((unsigned)f2bf(v[0]) | ((unsigned)f2bf(v[1]) << 16), (unsigned)f2bf(v[2]) | ((unsigned)f2bf(v[3]) << 16));
+}
+__device__ __forceinline__ void st4(f16_t* p, const float* v) {
+  typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+  *(v4h*)p = (v4h){(f16_t)v[0], (f16_t)v[1], (f16_t)v[2], (f16_t)v[3]};
+}
+
+template <typename T, int D> struct Cfg {
+  static constexpr int ES = sizeof(T);
+  // LDS row pitch (elements): 16-byte reads of 8 consecutive rows and the 4-row x 32-byte blocks of a transposing read fall into
+  // different banks
+  static constexpr int LDP = ES == 4 ? D + 4 : D == 32 ? 56 : D == 64 ? 72 : D == 96 ? 104 : 144;
+  static constexpr int PPR = D * ES / 16, EPP = 16 / ES;       // 16-byte pieces of a row, elements of a piece
+  static constexpr int KK = D / 16, DT = D / 32, CP = D + 4;   // k steps, output tiles, fp32 pitch of the merge tile
+};
+
+// k-major operand of the second product: 16 streamed rows from row0 on (k slots in the order of the accumulator registers: 4 h .. 4 h + 3,
+// 8 + 4 h .. 8 + 4 h + 3 of lane half h), channels col0 + (lane & 31)
+template <typename T, int D> __device__ __forceinline__ Frag8<T> tr_frag(const T* tile, int row0, int col0, int lane) {
+  const int r = lane & 15, h = lane >> 5;
+  return tr_pair<8 * Cfg<T, D>::LDP, T>(tile + (row0 + 4 * h + (r >> 2)) * Cfg<T, D>::LDP + col0 + 16 * ((lane >> 4) & 1) + 4 * (r & 3));
+}
+#define TR_F32(D) template <> __device__ __forceinline__ Frag8<float> tr_frag<float, D>(const float* tile, int row0, int col0, int lane) { \
+    constexpr int P = Cfg<float, D>::LDP; \
+    const float* p = tile + (row0 + 4 * (lane >> 5)) * P + col0 + (lane & 31); \
+    Frag8<float> f; \
+    f.v[0] = p[0]; f.v[1] = p[P]; f.v[2] = p[2 * P]; f.v[3] = p[3 * P]; f.v[4] = p[8 * P]; f.v[5] = p[9 * P]; f.v[6] = p[10 * P]; f.v[7] = p[11 * P]; \
+    return f; }
+TR_F32(32) TR_F32(64) TR_F32(96) TR_F32(128)
+#undef TR_F32
+
+struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
+struct WinArgs {
+  Mat q, k, v, o, go, dq, dk, dv;
+  float *lse, *delta, *part;
+  const int *starts, *lens;
+  int kv, group, Nq, Nk, rows, left, right, sinks, start, tiles, nsplit, sink_tiles, nchunk, g_f32;
+  float c, scale;
+};
+
+// contiguous ranges of the (batch, key head, tile) space per XCD: the blocks of one XCD's L2 read the same keys
+__device__ __forceinline__ int xcd_range(int id, int total) {
+  const int q = total >> 3, rem = total & 7, x = id & 7;
+  return x * q + min(x, rem) + (id >> 3);
+}
+
+struct Seq { int start, len; };
+__device__ __forceinline__ Seq sequence(const WinArgs& a, int b) {
+  Seq s;
+  s.len = a.lens ? min(max(a.lens[b], 0), a.Nk) : a.Nk;
+  s.start = a.starts ? min(max(a.starts[b], -FAR), FAR) : a.start;
+  return s;
+}
+
+// 32 * KS keys of a matrix, zeros behind `len`: global -> registers -> LDS, by NTH threads
+template <typename T, int D, int KT, int NTH> struct Stage {
+  using C = Cfg<T, D>;
+  static constexpr int NP = KT * C::PPR / NTH;
+  static_assert(NP * NTH == KT * C::PPR, "every piece of a tile has a thread");
+  v4u r[NP];
+  __device__ __forceinline__ void load(const T* base, int64_t st, int k0, int len, int gid) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int idx = gid + i * NTH, row = idx / C::PPR, c = idx % C::PPR, key = k0 + row;
+      r[i] = (v4u){0, 0, 0, 0};
+      if (key < len) r[i] = *(const v4u*)(base + (int64_t)key * st + c * C::EPP);
+    }
+  }
+  __device__ __forceinline__ void load_rows(const T* base, int64_t st, int64_t sh, int group, int r0, int rlo, int rhi, int gid) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int idx = gid + i * NTH, row = r0 + idx / C::PPR, c = idx % C::PPR;
+      r[i] = (v4u){0, 0, 0, 0};
+      if (row >= rlo && row < rhi) {
+        const int t = group == 1 ? row : row / group;
+        r[i] = *(const v4u*)(base + (int64_t)t * st + (int64_t)(row - t * group) * sh + c * C::EPP);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* dst, int gid) const {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int idx = gid + i * NTH, row = idx / C::PPR, c = idx % C::PPR;
+      *(v4u*)(dst + row * C::LDP + c * C::EPP) = r[i];
+    }
+  }
+};
+
+// a wave's own LDS writes before its own reads (no other wave is concerned)
+__device__ __forceinline__ void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+template <typename T, int D, bool WIDE> struct Shape {
+  using C = Cfg<T, D>;
+  // WIDE: four waves own 32 rows each and share every staged tile (two LDS buffers, one barrier per tile).  Otherwise all four own the same
+  // 32 rows, stream different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
+  static constexpr int KS = (WIDE && C::ES == 2) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64, NBUF = WIDE ? 2 : 1;
+  static constexpr size_t tile = (size_t)KT * C::LDP * C::ES;
+  static constexpr size_t stage = WIDE ? 2 * NBUF * tile : 4 * 2 * tile;
+  static constexpr size_t merge = WIDE ? 0 : (size_t)4 * 32 * C::CP * 4;
+  static constexpr size_t big = stage > merge ? stage : merge;
+  static constexpr size_t fwd = big + (WIDE ? 0 : 2 * 4 * 32 * 4);
+  // dK / dV: tiles of query rows
+  static constexpr int QS = (WIDE && C::ES == 2 && D <= 96) ? 2 : 1, RT = 32 * QS;
+  static constexpr size_t rtile = (size_t)RT * C::LDP * C::ES;
+  static constexpr size_t rstage = (WIDE ? NBUF : 4) * (2 * rtile + 2 * RT * 4);
+  static constexpr size_t kvb = rstage > merge ? rstage : merge;
+};
+
+// the tiles of KT keys that rows at positions [p0, p1] see at all: `nsink` from key 0 on, then from tile w0 on, nt in all
+struct Plan { int nsink, w0, nt; };
+template <int KT> __device__ __forceinline__ Plan key_tiles(const WinArgs& a, int len, int p0, int p1) {
+  Plan k{0, 0, 0};
+  p0 = max(p0, 0); p1 = min(p1, len - 1);
+  if (p0 > p1) return k;
+  const int lo = max(0, p0 - a.left), hi = min(len - 1, p1 + a.right);
+  k.w0 = lo / KT;
+  k.nsink = min((min(a.sinks, len) + KT - 1) / KT, k.w0);
+  k.nt = k.nsink + hi / KT - k.w0 + 1;
+  return k;
+}
+
+// what one lane's query row may see: keys [.., hi] that are >= lo or a sink
+struct Row { int r, i, g, p, lo, hi; bool live; };
+__device__ __forceinline__ Row row_of(const WinArgs& a, const Seq& s, int r) {
+  Row w;
+  w.r = r;
+  const int rc = min(r, a.rows - 1);
+  w.i = rc / a.group; w.g = rc - w.i * a.group; w.p = s.start + w.i;
+  w.live = r < a.rows && w.p >= 0 && w.p < s.len;
+  w.hi = w.live ? min(w.p + a.right, s.len - 1) : -1;
+  w.lo = w.live ? w.p - a.left : 0;
+  return w;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(256) void k_win_fwd(const WinArgs a) {
+  using C = Cfg<T, D>;
+  using S = Shape<T, D, WIDE>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, h = lane >> 5;
+  int flat = xcd_range(blockIdx.x, gridDim.x);
+  const int split = flat % a.nsplit; flat /= a.nsplit;
+  const int bh = flat / a.tiles, tile = flat % a.tiles, b = bh / a.kv, kvh = bh % a.kv, r0 = tile * S::ROWS;
+  const Seq sq = sequence(a, b);
+  const int wr0 = WIDE ? r0 + 32 * wv : r0;
+  const Row row = row_of(a, sq, wr0 + c32);
+  const T* Kb = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)kvh * a.k.h;
+  const T* Vb = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)kvh * a.v.h;
+  const T* Qr = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)row.i * a.q.t + (int64_t)(kvh * a.group + row.g) * a.q.h;
+  Frag8<T> qf[C::KK];
+#pragma unroll
+  for (int kk = 0; kk < C::KK; kk++) qf[kk] = ldg8(Qr + 16 * kk + 8 * h);
+  v16f acc[C::DT];
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
+  float m = -INFINITY, mc = 0.f, l = 0.f;
+  const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
+  const int per = (pl.nt + a.nsplit - 1) / a.nsplit, t1 = min(pl.nt, (split + 1) * per);
+  // positions of the wave's first and last row (none: nothing to compute, but its threads stage for the others)
+  const bool rows_here = wr0 < a.rows;
+  const int pw0 = sq.start + wr0 / a.group, pw1 = sq.start + min(wr0 + 31, a.rows - 1) / a.group;
+  auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
+
+  auto compute = [&](const T* ks, const T* vs, int k0) {
+    const bool none = !rows_here || k0 > pw1 + a.right || (k0 + S::KT - 1 < pw0 - a.left && k0 >= a.sinks);
+    if (none) return;
+    const bool all = k0 + S::KT - 1 <= min(pw0 + a.right, sq.len - 1) && (k0 >= pw1 - a.left || k0 + S::KT <= a.sinks);
+    v16f s[S::KS];
+#pragma unroll
+    for (int u = 0; u < S::KS; u++) {
+      s[u] = zero16();
+#pragma unroll
+      for (int kk = 0; kk < C::KK; kk++) s[u] = mma32(frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), qf[kk], s[u]);
+    }
+    if (!all) {
+#pragma unroll
+      for (int u = 0; u < S::KS; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int j = k0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+          s[u][i] = (j <= row.hi && (j >= row.lo || j < a.sinks)) ? s[u][i] : -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < S::KS; u++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx);
+    if (__builtin_amdgcn_ballot_w64(mn > m)) {        // (the maximum of a row moves in its first tiles, hardly ever after them)
+      // (alpha from the rounded products: exactly 1 for the rows whose maximum stays, whatever the wave's other rows hold)
+      const float nc = mn == -INFINITY ? 0.f : mn * a.c, alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - nc);
+      m = mn; mc = nc; l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++) acc[dt] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < S::KS; u++)
+#pragma unroll
+      for (int st = 0; st < 2; st++) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * st + i], a.c, -mc)); l += p[i]; }
+        const Frag8<T> pf = pack8(p, T{});
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(tr_frag<T, D>(vs, 32 * u + 16 * st, 32 * dt, lane), pf, acc[dt]);
+      }
+  };
+
+  Stage<T, D, S::KT, S::NTH> sk, sv;
+  if (WIDE) {
+    int t = split * per, buf = 0;
+    T* base = (T*)smem;
+    auto kbuf = [&](int i) { return base + i * 2 * S::KT * C::LDP; };
+    if (t < t1) {
+      sk.load(Kb, a.k.t, key_of(t), sq.len, tid); sv.load(Vb, a.v.t, key_of(t), sq.len, tid);
+      sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
+    }
+    lds_barrier();
+    for (; t < t1; t++) {
+      const bool more = t + 1 < t1;
+      if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
+      compute(kbuf(buf), kbuf(buf) + S::KT * C::LDP, key_of(t));
+      if (more) { sk.store(kbuf(buf ^ 1), tid); sv.store(kbuf(buf ^ 1) + S::KT * C::LDP, tid); }
+      lds_barrier();
+      buf ^= 1;
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (row.r < a.rows) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* Or = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)row.i * a.o.t + (int64_t)(kvh * a.group + row.g) * a.o.h;
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[j] = row.live ? acc[dt][4 * q + j] * inv : 0.f;
+          st4(Or + 32 * dt + 8 * q + 4 * h, v);
+        }
+      if (h == 0 && a.lse) a.lse[(int64_t)bh * a.rows + row.r] = row.live && l != 0.f ? mc + __builtin_amdgcn_logf(l) : INFINITY;
+    }
+    return;
+  }
+
+  T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
+  T* vs = ks + S::KT * C::LDP;
+  int t = split * per + wv;
+  if (t < t1) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
+  for (; t < t1; t += 4) {
+    sk.store(ks, lane); sv.store(vs, lane);
+    wave_lds_sync();
+    if (t + 4 < t1) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
+    compute(ks, vs, key_of(t));
+    wave_lds_sync();
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!row.live) { l = 0.f; m = -INFINITY; }
+  float* part = (float*)smem;
+  float* mw = (float*)(smem + S::big);
+  float* lw = mw + 4 * 32;
+  __syncthreads();      // every wave is done with its tiles
+  if (h == 0) { mw[wv * 32 + c32] = m == -INFINITY ? -INFINITY : mc; lw[wv * 32 + c32] = l; }
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = row.live ? acc[dt][4 * q + j] : 0.f;
+      st4(part + (wv * 32 + c32) * C::CP + 32 * dt + 8 * q + 4 * h, v);
+    }
+  __syncthreads();
+  for (int idx = tid; idx < 32 * (D / 4); idx += 256) {
+    const int rr = idx / (D / 4), c4 = idx % (D / 4), r = r0 + rr;
+    if (r >= a.rows) break;      // (rows only grow with idx)
+    float M = mw[rr];
+#pragma unroll
+    for (int w = 1; w < 4; w++) M = fmaxf(M, mw[w * 32 + rr]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float e = __builtin_amdgcn_exp2f(mw[w * 32 + rr] - Ms);
+      const v4f x = *(const v4f*)(part + (w * 32 + rr) * C::CP + 4 * c4);
+      L += lw[w * 32 + rr] * e;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] += x[j] * e;
+    }
+    if (a.nsplit > 1) {
+      float* ws = a.part + ((int64_t)(bh * a.nsplit + split) * a.rows + r) * (D + 4);
+      st4(ws + 4 * c4, v);
+      if (c4 == 0) { ws[D] = M; ws[D + 1] = L; }
+      continue;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int i = r / a.group, g = r - i * a.group;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] *= inv;
+    st4((T*)a.o.p + (int64_t)b * a.o.b + (int64_t)i * a.o.t + (int64_t)(kvh * a.group + g) * a.o.h + 4 * c4, v);
+    if (c4 == 0 && a.lse) a.lse[(int64_t)bh * a.rows + r] = L != 0.f ? Ms + __builtin_amdgcn_logf(L) : INFINITY;
+  }
+}
+
+// few rows, many keys: the shares of the key tiles of one row, merged in share order
+template <typename T, int D>
+__global__ __launch_bounds__(64) void k_win_merge(const WinArgs a) {
+  const int bh = blockIdx.y, r = blockIdx.x, lane = threadIdx.x, b = bh / a.kv, kvh = bh % a.kv;
+  const float* ws = a.part + ((int64_t)bh * a.nsplit * a.rows + r) * (D + 4);
+  const int64_t step = (int64_t)a.rows * (D + 4);
+  float M = -INFINITY;
+  for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, ws[s * step + D]);
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f, v[2] = {0.f, 0.f};
+  for (int s = 0; s < a.nsplit; s++) {
+    const float* p = ws + s * step;
+    const float e = __builtin_amdgcn_exp2f(p[D] - Ms);
+    L += p[D + 1] * e;
+#pragma unroll
+    for (int k = 0; k < 2; k++) if (lane + 64 * k < D) v[k] += p[lane + 64 * k] * e;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int i = r / a.group, g = r - i * a.group;
+  T* o = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)i * a.o.t + (int64_t)(kvh * a.group + g) * a.o.h;
+#pragma unroll
+  for (int k = 0; k < 2; k++) if (lane + 64 * k < D) st_f(o + lane + 64 * k, v[k] * inv);
+  if (lane == 0 && a.lse) a.lse[(int64_t)bh * a.rows + r] = L != 0.f ? Ms + __builtin_amdgcn_logf(L) : INFINITY;
+}
+
+template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t off, int f32, const float* v) {
+  if (f32) st4((float*)p + off, v); else st4((T*)p + off, v);
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ (and delta)
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(256) void k_win_dq(const WinArgs a) {
+  using C = Cfg<T, D>;
+  using S = Shape<T, D, WIDE>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, h = lane >> 5;
+  const int flat = xcd_range(blockIdx.x, gridDim.x);
+  const int bh = flat / a.tiles, tile = flat % a.tiles, b = bh / a.kv, kvh = bh % a.kv, r0 = tile * S::ROWS;
+  const Seq sq = sequence(a, b);
+  const int wr0 = WIDE ? r0 + 32 * wv : r0;
+  const Row row = row_of(a, sq, wr0 + c32);
+  const int head = kvh * a.group + row.g;
+  const T* Kb = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)kvh * a.k.h;
+  const T* Vb = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)kvh * a.v.h;
+  const T* Qr = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)row.i * a.q.t + (int64_t)head * a.q.h;
+  const T* Gr = (const T*)a.go.p + (int64_t)b * a.go.b + (int64_t)row.i * a.go.t + (int64_t)head * a.go.h;
+  const T* Or = (const T*)a.o.p + (int64_t)b * a.o.b + (int64_t)row.i * a.o.t + (int64_t)head * a.o.h;
+  Frag8<T> qf[C::KK], gf[C::KK];
+  float dl = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < C::KK; kk++) {
+    qf[kk] = ldg8(Qr + 16 * kk + 8 * h); gf[kk] = ldg8(Gr + 16 * kk + 8 * h);
+    const Frag8<T> of = ldg8(Or + 16 * kk + 8 * h);
+#pragma unroll
+    for (int i = 0; i < 8; i++) dl += elem(of, i) * elem(gf[kk], i);
+  }
+  dl += __shfl_xor(dl, 32, 64);
+  const float lse = row.live ? a.lse[(int64_t)bh * a.rows + row.r] : INFINITY;
+  if (row.r < a.rows && h == 0 && (WIDE || wv == 0)) a.delta[(int64_t)bh * a.rows + row.r] = row.live ? dl : 0.f;
+  const float ds0 = -dl * a.scale;
+  v16f acc[C::DT];
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
+  const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
+  const bool rows_here = wr0 < a.rows;
+  const int pw0 = sq.start + wr0 / a.group, pw1 = sq.start + min(wr0 + 31, a.rows - 1) / a.group;
+  auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
+
+  auto compute = [&](const T* ks, const T* vs, int k0) {
+    const bool none = !rows_here || k0 > pw1 + a.right || (k0 + S::KT - 1 < pw0 - a.left && k0 >= a.sinks);
+    if (none) return;
+    const bool all = k0 + S::KT - 1 <= min(pw0 + a.right, sq.len - 1) && (k0 >= pw1 - a.left || k0 + S::KT <= a.sinks);
+#pragma unroll
+    for (int u = 0; u < S::KS; u++) {
+      v16f s = zero16(), dp = zero16();
+#pragma unroll
+      for (int kk = 0; kk < C::KK; kk++) {
+        s = mma32(frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), qf[kk], s);
+        dp = mma32(frag_ld_lds(vs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), gf[kk], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, ds0);
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int j = k0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+          s[i] = (j <= row.hi && (j >= row.lo || j < a.sinks)) ? s[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; st++) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = s[8 * st + i];
+        const Frag8<T> pf = pack8(p, T{});
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(tr_frag<T, D>(ks, 32 * u + 16 * st, 32 * dt, lane), pf, acc[dt]);
+      }
+    }
+  };
+
+  Stage<T, D, S::KT, S::NTH> sk, sv;
+  const int64_t qoff = (int64_t)b * a.dq.b + (int64_t)row.i * a.dq.t + (int64_t)head * a.dq.h;
+  if (WIDE) {
+    int t = 0, buf = 0;
+    T* base = (T*)smem;
+    auto kbuf = [&](int i) { return base + i * 2 * S::KT * C::LDP; };
+    if (t < pl.nt) {
+      sk.load(Kb, a.k.t, key_of(t), sq.len, tid); sv.load(Vb, a.v.t, key_of(t), sq.len, tid);
+      sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
+    }
+    lds_barrier();
+    for (; t < pl.nt; t++) {
+      const bool more = t + 1 < pl.nt;
+      if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
+      compute(kbuf(buf), kbuf(buf) + S::KT * C::LDP, key_of(t));
+      if (more) { sk.store(kbuf(buf ^ 1), tid); sv.store(kbuf(buf ^ 1) + S::KT * C::LDP, tid); }
+      lds_barrier();
+      buf ^= 1;
+    }
+    if (row.r < a.rows) {
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) v[j] = row.live ? acc[dt][4 * q + j] : 0.f;
+          st4_grad<T>(a.dq.p, qoff + 32 * dt + 8 * q + 4 * h, a.g_f32, v);
+        }
+    }
+    return;
+  }
+  T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
+  T* vs = ks + S::KT * C::LDP;
+  int t = wv;
+  if (t < pl.nt) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
+  for (; t < pl.nt; t += 4) {
+    sk.store(ks, lane); sv.store(vs, lane);
+    wave_lds_sync();
+    if (t + 4 < pl.nt) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
+    compute(ks, vs, key_of(t));
+    wave_lds_sync();
+  }
+  float* part = (float*)smem;
+  __syncthreads();
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = row.live ? acc[dt][4 * q + j] : 0.f;
+      st4(part + (wv * 32 + c32) * C::CP + 32 * dt + 8 * q + 4 * h, v);
+    }
+  __syncthreads();
+  for (int idx = tid; idx < 32 * (D / 4); idx += 256) {
+    const int rr = idx / (D / 4), c4 = idx % (D / 4), r = r0 + rr;
+    if (r >= a.rows) break;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const v4f x = *(const v4f*)(part + (w * 32 + rr) * C::CP + 4 * c4);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] += x[j];
+    }
+    const int i = r / a.group, g = r - i * a.group;
+    st4_grad<T>(a.dq.p, (int64_t)b * a.dq.b + (int64_t)i * a.dq.t + (int64_t)(kvh * a.group + g) * a.dq.h + 4 * c4, a.g_f32, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+// query rows [lo, hi) that see key j at all
+struct Span { int lo, hi; };
+__device__ __forceinline__ Span rows_of(const WinArgs& a, const Seq& s, int jlo, int jhi) {      // ... that see any key of [jlo, jhi], jhi < len
+  const int p0 = max(jlo - a.right, 0), p1 = jlo < a.sinks ? s.len - 1 : min(jhi + a.left, s.len - 1);
+  const int i0 = min(max(p0 - s.start, 0), a.Nq), i1 = min(p1 - s.start, a.Nq - 1);
+  return Span{i0 * a.group, i1 < i0 ? i0 * a.group : (i1 + 1) * a.group};
+}
+
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(256) void k_win_dkv(const WinArgs a) {
+  using C = Cfg<T, D>;
+  using S = Shape<T, D, WIDE>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, h = lane >> 5;
+  // the tiles that hold sinks are seen by (nearly) every row: their rows are dealt to nchunk blocks, added up afterwards
+  const int ktiles = (a.Nk + S::ROWS - 1) / S::ROWS, per_bh = a.sink_tiles * a.nchunk + ktiles - a.sink_tiles;
+  const int flat = xcd_range(blockIdx.x, gridDim.x), bh = flat / per_bh, e = flat % per_bh, b = bh / a.kv, kvh = bh % a.kv;
+  const bool shared_rows = e < a.sink_tiles * a.nchunk && a.nchunk > 1;
+  const int tile = e < a.sink_tiles * a.nchunk ? e / a.nchunk : e - a.sink_tiles * (a.nchunk - 1), chunk = shared_rows ? e % a.nchunk : 0;
+  const int k0 = tile * S::ROWS;
+  const Seq sq = sequence(a, b);
+  const int j = k0 + (WIDE ? 32 * wv : 0) + c32;
+  const bool live = j < sq.len;
+  const T* Qb = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)kvh * a.group * a.q.h;
+  const T* Gb = (const T*)a.go.p + (int64_t)b * a.go.b + (int64_t)kvh * a.group * a.go.h;
+  const float *lseb = a.lse + (int64_t)bh * a.rows, *dlb = a.delta + (int64_t)bh * a.rows;
+  Frag8<T> kf[C::KK], vf[C::KK];
+  {
+    const int jc = live ? j : 0;       // (a key behind the sequence: any key, its column is thrown away)
+    const T* Kr = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)jc * a.k.t + (int64_t)kvh * a.k.h;
+    const T* Vr = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)jc * a.v.t + (int64_t)kvh * a.v.h;
+#pragma unroll
+    for (int kk = 0; kk < C::KK; kk++) { kf[kk] = ldg8(Kr + 16 * kk + 8 * h); vf[kk] = ldg8(Vr + 16 * kk + 8 * h); }
+  }
+  v16f ak[C::DT], av[C::DT];
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) { ak[dt] = zero16(); av[dt] = zero16(); }
+  const Span mine = live ? rows_of(a, sq, j, j) : Span{0x7fffffff, 0};
+  const Span block = k0 < sq.len ? rows_of(a, sq, k0, min(k0 + S::ROWS, sq.len) - 1) : Span{0, 0};
+  // (rows that all keys of the wave see need no mask, rows that none of them sees no work)
+  int all_lo = mine.lo, all_hi = mine.hi, any_lo = mine.lo, any_hi = mine.hi;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all_lo = max(all_lo, __shfl_xor(all_lo, o, 64)); all_hi = min(all_hi, __shfl_xor(all_hi, o, 64));
+    any_lo = min(any_lo, __shfl_xor(any_lo, o, 64)); any_hi = max(any_hi, __shfl_xor(any_hi, o, 64));
+  }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  any_lo = __builtin_amdgcn_readfirstlane(any_lo); any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+  const int base_r = block.lo / S::RT * S::RT, ntile = block.hi > block.lo ? (block.hi - base_r + S::RT - 1) / S::RT : 0;
+  const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t1 = min(ntile, (chunk + 1) * per);
+
+  auto compute = [&](const T* qs, const T* gs, const float* sl, const float* sd, int rt) {
+#pragma unroll
+    for (int u = 0; u < S::QS; u++) {
+      const int r0 = rt + 32 * u;
+      if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
+      const bool all = r0 >= all_lo && r0 + 32 <= all_hi;
+      v16f s = zero16(), dp = zero16();
+#pragma unroll
+      for (int kk = 0; kk < C::KK; kk++) {
+        s = mma32(frag_ld_lds(qs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), kf[kk], s);
+        dp = mma32(frag_ld_lds(gs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), vf[kk], dp);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const v4f ls = *(const v4f*)(sl + 32 * u + 8 * q + 4 * h), dl = *(const v4f*)(sd + 32 * u + 8 * q + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[4 * q + i], a.c, -ls[i])), d = p * fmaf(dp[4 * q + i], a.scale, -dl[i]);
+          if (!all) {
+            const int r = r0 + 8 * q + 4 * h + i;
+            const bool see = r >= mine.lo && r < mine.hi;
+            p = see ? p : 0.f; d = see ? d : 0.f;
+          }
+          s[4 * q + i] = p; dp[4 * q + i] = d;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; st++) {
+        float p[8], d[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) { p[i] = s[8 * st + i]; d[i] = dp[8 * st + i]; }
+        const Frag8<T> pf = pack8(p, T{}), df = pack8(d, T{});
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) {
+          av[dt] = mma32(tr_frag<T, D>(gs, 32 * u + 16 * st, 32 * dt, lane), pf, av[dt]);
+          ak[dt] = mma32(tr_frag<T, D>(qs, 32 * u + 16 * st, 32 * dt, lane), df, ak[dt]);
+        }
+      }
+    }
+  };
+
+  Stage<T, D, S::RT, S::NTH> sqr, sgr;
+  float ls = 0.f, dl = 0.f;
+  const int gid = WIDE ? tid : lane;
+  // rows outside [lo, hi) of the block are staged as zeros with an infinite lse: they add nothing, whatever they hold
+  auto load = [&](int rt) {
+    sqr.load_rows(Qb, a.q.t, a.q.h, a.group, rt, block.lo, block.hi, gid);
+    sgr.load_rows(Gb, a.go.t, a.go.h, a.group, rt, block.lo, block.hi, gid);
+    if (gid < S::RT) {
+      const int r = rt + gid;
+      const bool ok = r >= block.lo && r < block.hi;
+      ls = ok ? lseb[r] : INFINITY; dl = ok ? dlb[r] * a.scale : 0.f;
+    }
+  };
+  auto store = [&](T* qs, T* gs, float* sl, float* sd) {
+    sqr.store(qs, gid); sgr.store(gs, gid);
+    if (gid < S::RT) { sl[gid] = ls; sd[gid] = dl; }
+  };
+  constexpr size_t set = 2 * S::rtile + 2 * S::RT * 4;
+  auto qs_of = [&](int i) { return (T*)(smem + i * set); };
+  auto sl_of = [&](int i) { return (float*)(smem + i * set + 2 * S::rtile); };
+  float* ws = shared_rows ? a.part + (((int64_t)bh * a.sink_tiles + tile) * a.nchunk + chunk) * (2 * S::ROWS * D) : nullptr;
+  const int64_t koff = (int64_t)b * a.dk.b + (int64_t)kvh * a.dk.h, voff = (int64_t)b * a.dv.b + (int64_t)kvh * a.dv.h;
+  if (WIDE) {
+    int t = chunk * per, buf = 0;
+    if (t < t1) { load(base_r + t * S::RT); store(qs_of(0), qs_of(0) + S::RT * C::LDP, sl_of(0), sl_of(0) + S::RT); }
+    lds_barrier();
+    for (; t < t1; t++) {
+      const bool more = t + 1 < t1;
+      if (more) load(base_r + (t + 1) * S::RT);
+      compute(qs_of(buf), qs_of(buf) + S::RT * C::LDP, sl_of(buf), sl_of(buf) + S::RT, base_r + t * S::RT);
+      if (more) store(qs_of(buf ^ 1), qs_of(buf ^ 1) + S::RT * C::LDP, sl_of(buf ^ 1), sl_of(buf ^ 1) + S::RT);
+      lds_barrier();
+      buf ^= 1;
+    }
+    if (j < a.Nk) {
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          float x[4], y[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) { x[i] = live ? ak[dt][4 * q + i] : 0.f; y[i] = live ? av[dt][4 * q + i] : 0.f; }
+          const int ch = 32 * dt + 8 * q + 4 * h;
+          if (shared_rows) { st4(ws + (j - k0) * D + ch, x); st4(ws + (S::ROWS + j - k0) * D + ch, y); }
+          else { st4_grad<T>(a.dk.p, koff + (int64_t)j * a.dk.t + ch, a.g_f32, x); st4((T*)a.dv.p + voff + (int64_t)j * a.dv.t + ch, y); }
+        }
+    }
+    return;
+  }
+  int t = chunk * per + wv;
+  if (t < t1) load(base_r + t * S::RT);
+  for (; t < t1; t += 4) {
+    store(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT);
+    wave_lds_sync();
+    if (t + 4 < t1) load(base_r + (t + 4) * S::RT);
+    compute(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT, base_r + t * S::RT);
+    wave_lds_sync();
+  }
+  float* part = (float*)smem;
+#pragma unroll
+  for (int pass = 0; pass < 2; pass++) {
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < C::DT; dt++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = live ? (pass ? av[dt][4 * q + i] : ak[dt][4 * q + i]) : 0.f;
+        st4(part + (wv * 32 + c32) * C::CP + 32 * dt + 8 * q + 4 * h, x);
+      }
+    __syncthreads();
+    for (int idx = tid; idx < 32 * (D / 4); idx += 256) {
+      const int rr = idx / (D / 4), c4 = idx % (D / 4), key = k0 + rr;
+      if (key >= a.Nk) break;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const v4f x = *(const v4f*)(part + (w * 32 + rr) * C::CP + 4 * c4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += x[i];
+      }
+      if (shared_rows) st4(ws + (pass * S::ROWS + rr) * D + 4 * c4, v);
+      else if (pass) st4((T*)a.dv.p + voff + (int64_t)key * a.dv.t + 4 * c4, v);
+      else st4_grad<T>(a.dk.p, koff + (int64_t)key * a.dk.t + 4 * c4, a.g_f32, v);
+    }
+  }
+}
+
+// dK, dV of the keys whose rows were dealt to several blocks, added in block order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_win_sink_sum(const WinArgs a, int keys) {      // keys: rows of a tile
+  const int nb = (2 * keys * (D / 4) + 255) / 256, bt = blockIdx.x / nb, bh = bt / a.sink_tiles, tile = bt % a.sink_tiles, b = bh / a.kv, kvh = bh % a.kv;
+  const int idx = (blockIdx.x % nb) * 256 + threadIdx.x, which = idx / (keys * (D / 4)), rest = idx % (keys * (D / 4)), key = tile * keys + rest / (D / 4), ch = 4 * (rest % (D / 4));
+  if (which > 1 || key >= a.Nk) return;
+  const float* p = a.part + (int64_t)bt * a.nchunk * (2 * keys * D) + (int64_t)which * keys * D + (rest / (D / 4)) * D + ch;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < a.nchunk; c++) {
+    const v4f x = *(const v4f*)(p + (int64_t)c * (2 * keys * D));
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += x[i];
+  }
+  if (which) st4((T*)a.dv.p + (int64_t)b * a.dv.b + (int64_t)kvh * a.dv.h + (int64_t)key * a.dv.t + ch, v);
+  else st4_grad<T>(a.dk.p, (int64_t)b * a.dk.b + (int64_t)kvh * a.dk.h + (int64_t)key * a.dk.t + ch, a.g_f32, v);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int raise_lds(const void* kern, size_t smem, const char* name) {
+  if (smem > 48 * 1024) {
+    hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != hipSuccess) { (void)hipGetLastError(); DP_FAIL("%s: cannot raise dynamic LDS to %zu: %s", name, smem, hipGetErrorString(e)); }
+  }
+  return 0;
+}
+
+// Which kernel, how many blocks: decided by sizes alone.
+struct Launch { bool wide; int tiles, nsplit; bool kwide; int ktiles, sink_tiles, nchunk; };
+Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right, int sinks) {
+  Launch p;
+  const int64_t rows = Nq > 0 ? (int64_t)Nq * group : 1, bk = (int64_t)B * kv;
+  p.wide = (rows + 127) / 128 * bk >= 256;
+  p.tiles = (int)((rows + (p.wide ? 127 : 31)) / (p.wide ? 128 : 32));
+  p.nsplit = 1;
+  const int64_t span = left >= FAR || right >= FAR ? Nk : (int64_t)left + right + sinks + 32;
+  const int64_t rounds = ((span < Nk ? span : Nk) + 127) / 128;      // 32-key tiles for each of the four waves
+  if (!p.wide && p.tiles * bk < 256) {
+    int64_t n = 512 / (p.tiles * bk);
+    if (n > rounds / 4) n = rounds / 4;
+    p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  }
+  p.kwide = (int64_t)(Nk + 127) / 128 * bk >= 256;
+  const int kb = p.kwide ? 128 : 32;
+  p.ktiles = (Nk + kb - 1) / kb;
+  p.sink_tiles = 0; p.nchunk = 1;
+  if (sinks > 0 && left < FAR && Nk > 0) {
+    const int64_t usual = ((int64_t)left + (right >= FAR ? Nk : right) + kb) * group;      // rows of any other tile
+    int64_t n = rows / (usual < 512 ? 512 : usual);
+    const int64_t st = ((sinks < Nk ? sinks : Nk) + kb - 1) / kb, most = (64ll << 20) / (bk * st * 2 * kb * d);      // (256 MB of partial sums at most)
+    if (n > most) n = most;
+    p.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    if (p.nchunk > 1) p.sink_tiles = (int)st;
+  }
+  return p;
+}
+
+int check(const char* name, int B, int heads, int kv, int Nq, int Nk, int d, int left, int right, int sinks, float scale, int dtype) {
+  if (dtype != DP_F32 && dtype != DP_BF16 && dtype != DP_F16) DP_FAIL("%s: bad dtype %d", name, dtype);
+  if (d != 32 && d != 64 && d != 96 && d != 128) DP_FAIL("%s: head dim %d not in {32, 64, 96, 128}", name, d);
+  if (B < 0 || heads < 1 || kv < 1 || heads % kv || Nq < 0 || Nk < 0) DP_FAIL("%s: bad sizes B=%d heads=%d/%d Nq=%d Nk=%d", name, B, heads, kv, Nq, Nk);
+  if (left < -1 || right < -1 || sinks < 0) DP_FAIL("%s: bad window left=%d right=%d sinks=%d", name, left, right, sinks);
+  if (!(scale > 0.f) || !(scale < 1e30f)) DP_FAIL("%s: scale %g", name, (double)scale);
+  if (Nk >= FAR / 2 || (int64_t)Nq * (heads / kv) >= FAR / 2 || (int64_t)B * kv * ((Nk > Nq * (int64_t)(heads / kv) ? Nk : Nq * (int64_t)(heads / kv)) / 32 + 64) >= FAR)
+    DP_FAIL("%s: too many rows", name);
+  return 0;
+}
+int check_mat(const char* name, const char* what, const Mat& m, int es) {
+  if (((uintptr_t)m.p & 15) || (m.b * es) % 16 || (m.t * es) % 16 || (m.h * es) % 16) DP_FAIL("%s: %s: rows must be 16-byte aligned", name, what);
+  return 0;
+}
+
+template <typename T, int D, bool WIDE> int run_fwd(const WinArgs& a, int B, hipStream_t st) {
+  auto kern = k_win_fwd<T, D, WIDE>;
+  constexpr size_t smem = Shape<T, D, WIDE>::fwd;
+  static_assert(smem <= 160 * 1024, "LDS of a CU");
+  if (raise_lds((const void*)kern, smem, "window_attention_fwd")) return 1;
+  hipLaunchKernelGGL(kern, dim3(a.tiles * a.nsplit * B * a.kv), dim3(256), smem, st, a);
+  DP_CHECK_LAUNCH("window_attention_fwd");
+  if (a.nsplit > 1) {
+    hipLaunchKernelGGL((k_win_merge<T, D>), dim3(a.rows, B * a.kv), dim3(64), 0, st, a);
+    DP_CHECK_LAUNCH("window_attention_fwd(merge)");
+  }
+  return 0;
+}
+template <typename T, int D, bool WIDE> int run_dq(const WinArgs& a, int B, hipStream_t st) {
+  auto kern = k_win_dq<T, D, WIDE>;
+  constexpr size_t smem = Shape<T, D, WIDE>::big;
+  if (raise_lds((const void*)kern, smem, "window_attention_bwd")) return 1;
+  hipLaunchKernelGGL(kern, dim3(a.tiles * B * a.kv), dim3(256), smem, st, a);
+  DP_CHECK_LAUNCH("window_attention_bwd(dq)");
+  return 0;
+}
+template <typename T, int D, bool WIDE> int run_dkv(const WinArgs& a, int B, int ktiles, hipStream_t st) {
+  auto kern = k_win_dkv<T, D, WIDE>;
+  constexpr size_t smem = Shape<T, D, WIDE>::kvb;
+  static_assert(smem <= 160 * 1024, "LDS of a CU");
+  if (raise_lds((const void*)kern, smem, "window_attention_bwd")) return 1;
+  hipLaunchKernelGGL(kern, dim3((a.sink_tiles * (a.nchunk - 1) + ktiles) * B * a.kv), dim3(256), smem, st, a);
+  DP_CHECK_LAUNCH("window_attention_bwd(dkv)");
+  if (a.sink_tiles) {
+    constexpr int keys = Shape<T, D, WIDE>::ROWS;
+    hipLaunchKernelGGL((k_win_sink_sum<T, D>), dim3(cdiv(2 * keys * (D / 4), 256) * a.sink_tiles * B * a.kv), dim3(256), 0, st, a, keys);
+    DP_CHECK_LAUNCH("window_attention_bwd(sinks)");
+  }
+  return 0;
+}
+
+}  // namespace
+
+#define WIN_DIMS(d, ...) do { if ((d) == 32) { constexpr int D = 32; __VA_ARGS__; } else if ((d) == 64) { constexpr int D = 64; __VA_ARGS__; } \
+    else if ((d) == 96) { constexpr int D = 96; __VA_ARGS__; } else { constexpr int D = 128; __VA_ARGS__; } } while (0)
+
+extern "C" int64_t dp_window_attention_ws_elems(int B, int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int backward) {
+  if (B < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || Nq < 1 || Nk < 1 || left < -1 || right < -1 || sinks < 0) return 0;
+  const int group = heads / kv_heads;
+  const Launch p = plan(B, kv_heads, group, Nq, Nk, d, left < 0 ? FAR : left, right < 0 ? FAR : right, sinks);
+  const int64_t bk = (int64_t)B * kv_heads;
+  if (!backward) return p.nsplit > 1 ? bk * p.nsplit * Nq * group * (d + 4) : 0;
+  return bk * p.sink_tiles * p.nchunk * 2 * (p.kwide ? 128 : 32) * d;
+}
+
+extern "C" int dp_window_attention_fwd(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* k, int64_t kb, int64_t kt, int64_t kh, const void* v,
+                                       int64_t vb, int64_t vt, int64_t vh, void* o, int64_t ob, int64_t ot, int64_t oh, float* lse, float* ws, int B,
+                                       int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int q_start, const int32_t* q_starts,
+                                       const int32_t* lengths, float scale, int dtype, void* stream) {
+  if (check("window_attention_fwd", B, heads, kv_heads, Nq, Nk, d, left, right, sinks, scale, dtype)) return 1;
+  WinArgs a{};
+  a.q = Mat{(void*)q, qb, qt, qh}; a.k = Mat{(void*)k, kb, kt, kh}; a.v = Mat{(void*)v, vb, vt, vh}; a.o = Mat{o, ob, ot, oh};
+  const int es = dtype == DP_F32 ? 4 : 2;
+  if (check_mat("window_attention_fwd", "q", a.q, es) || check_mat("window_attention_fwd", "k", a.k, es) || check_mat("window_attention_fwd", "v", a.v, es) ||
+      check_mat("window_attention_fwd", "o", a.o, es)) return 1;
+  if (B == 0 || Nq == 0) return 0;
+  a.lse = lse; a.part = ws; a.starts = q_starts; a.lens = lengths;
+  a.kv = kv_heads; a.group = heads / kv_heads; a.Nq = Nq; a.Nk = Nk; a.rows = Nq * a.group;
+  a.left = left < 0 ? FAR : left < FAR ? left : FAR; a.right = right < 0 ? FAR : right < FAR ? right : FAR; a.sinks = sinks < FAR ? sinks : FAR;
+  a.start = q_start < -FAR ? -FAR : q_start > FAR ? FAR : q_start;
+  a.scale = scale; a.c = scale * LOG2E;
+  const Launch p = plan(B, kv_heads, a.group, Nq, Nk, d, a.left, a.right, a.sinks);
+  a.tiles = p.tiles; a.nsplit = p.nsplit; a.nchunk = 1;
+  if (p.nsplit > 1 && (!ws || ((uintptr_t)ws & 15))) DP_FAIL("window_attention_fwd: needs a 16-byte aligned workspace (dp_window_attention_ws_elems)");
+  DP_DISPATCH(dtype, WIN_DIMS(d, return p.wide ? run_fwd<T, D, true>(a, B, STREAM) : run_fwd<T, D, false>(a, B, STREAM)));
+  return 0;
+}
+
+extern "C" int dp_window_attention_bwd(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* k, int64_t kb, int64_t kt, int64_t kh, const void* v,
+                                       int64_t vb, int64_t vt, int64_t vh, const void* o, int64_t ob, int64_t ot, int64_t oh, const void* go, int64_t gb,
+                                       int64_t gt, int64_t gh, const float* lse, float* delta, void* dq, int64_t dqb, int64_t dqt, int64_t dqh, void* dk,
+                                       int64_t dkb, int64_t dkt, int64_t dkh, void* dv, int64_t dvb, int64_t dvt, int64_t dvh, int qk_f32, float* ws, int B,
+                                       int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int q_start, const int32_t* q_starts,
+                                       const int32_t* lengths, float scale, int dtype, void* stream) {
+  const char* name = "window_attention_bwd";
+  if (check(name, B, heads, kv_heads, Nq, Nk, d, left, right, sinks, scale, dtype)) return 1;
+  WinArgs a{};
+  a.q = Mat{(void*)q, qb, qt, qh}; a.k = Mat{(void*)k, kb, kt, kh}; a.v = Mat{(void*)v, vb, vt, vh}; a.o = Mat{(void*)o, ob, ot, oh};
+  a.go = Mat{(void*)go, gb, gt, gh}; a.dq = Mat{dq, dqb, dqt, dqh}; a.dk = Mat{dk, dkb, dkt, dkh}; a.dv = Mat{dv, dvb, dvt, dvh};
+  const int es = dtype == DP_F32 ? 4 : 2, gs = qk_f32 ? 4 : es;
+  if (check_mat(name, "q", a.q, es) || check_mat(name, "k", a.k, es) || check_mat(name, "v", a.v, es) || check_mat(name, "o", a.o, es) ||
+      check_mat(name, "go", a.go, es) || check_mat(name, "dq", a.dq, gs) || check_mat(name, "dk", a.dk, gs) || check_mat(name, "dv", a.dv, es)) return 1;
+  if (B == 0) return 0;
+  if (Nq > 0 && (!lse || !delta)) DP_FAIL("%s: lse / delta missing", name);
+  a.lse = (float*)lse; a.delta = delta; a.part = ws; a.starts = q_starts; a.lens = lengths;
+  a.kv = kv_heads; a.group = heads / kv_heads; a.Nq = Nq; a.Nk = Nk; a.rows = Nq * a.group;
+  a.left = left < 0 ? FAR : left < FAR ? left : FAR; a.right = right < 0 ? FAR : right < FAR ? right : FAR; a.sinks = sinks < FAR ? sinks : FAR;
+  a.start = q_start < -FAR ? -FAR : q_start > FAR ? FAR : q_start;
+  a.scale = scale; a.c = scale * LOG2E; a.g_f32 = qk_f32 != 0;
+  const Launch p = plan(B, kv_heads, a.group, Nq, Nk, d, a.left, a.right, a.sinks);
+  a.tiles = p.tiles; a.nsplit = 1; a.sink_tiles = p.sink_tiles; a.nchunk = p.nchunk;
+  if (p.sink_tiles && (!ws || ((uintptr_t)ws & 15))) DP_FAIL("%s: needs a 16-byte aligned workspace (dp_window_attention_ws_elems)", name);
+  if (Nq > 0) {
+    int rc = 0;
+    DP_DISPATCH(dtype, WIN_DIMS(d, rc = p.wide ? run_dq<T, D, true>(a, B, STREAM) : run_dq<T, D, false>(a, B, STREAM)));
+    if (rc) return rc;
+  }
+  if (Nk == 0) return 0;
+  DP_DISPATCH(dtype, WIN_DIMS(d, return p.kwide ? run_dkv<T, D, true>(a, B, p.ktiles, STREAM) : run_dkv<T, D, false>(a, B, p.ktiles, STREAM)));
+  return 0;
+}

@@ -2331,6 +2331,351 @@ def attention(qkv, heads):
     return Attention.apply(qkv, heads)
 
 
+# ------------------------------------------------------------------------------------------------ rotary positions, norm of queries and keys
+_POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+HEAD_DIMS = (32, 64, 96, 128)
+
+
+def _device_of(t):
+    """Context in which launches go to t's device (nothing to do where it is the current one)."""
+    if _raw_device is not None and t.device.index == _raw_device():
+        return _NO_GUARD
+    return torch.cuda.device(t.device)
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _strided(t):
+    """(tensor, strides of all but the last dimension): t itself where its last dimension is dense and every row 16-byte aligned, otherwise a
+    contiguous copy."""
+    st, es = t.stride(), t.element_size()
+    if (st[-1] == 1 or t.shape[-1] <= 1) and t.data_ptr() % 16 == 0 and all(n <= 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], st)):
+        return t, [0 if n <= 1 else s for n, s in zip(t.shape[:-1], st)]
+    t = t.contiguous() if not t.is_contiguous() else t.clone()
+    return t, [0 if n <= 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+
+
+def _head_dim(width, heads, what):
+    if heads < 1 or width % heads:
+        raise ValueError(f"{what}: {width} channels do not divide into {heads} heads")
+    d = width // heads
+    if d not in HEAD_DIMS:
+        raise ValueError(f"{what}: head dim {d} not in {HEAD_DIMS}")
+    return d
+
+
+def _rotary_args(what, x, d, positions, sections, base, interleaved):
+    """(positions tensor, the C ABI's arguments behind the pointer) of a rotation; (None, ...) without one."""
+    if positions is None:
+        if sections is not None:
+            raise ValueError(f"{what}: sections without positions")
+        return None, (0, 0, 0, 0, 0, 0, 0, 0.0, 0)
+    if sections is None:
+        raise ValueError(f"{what}: positions need sections (rotated pairs of a head per axis)")
+    sections = tuple(int(s) for s in sections)
+    B, N = x.shape[:2]
+    if positions.dtype not in _POS_KIND:
+        raise TypeError(f"{what}: positions are int32, int64 or float32, got {positions.dtype}")
+    if positions.device != x.device:
+        raise _lib.DoseHipError(f"{what}: positions on {positions.device}, rows on {x.device}")
+    if positions.dim() not in (2, 3) or positions.shape[-2:] != (N, len(sections)) or (positions.dim() == 3 and positions.shape[0] not in (1, B)):
+        raise ValueError(f"{what}: positions {tuple(positions.shape)} for {B} x {N} tokens and {len(sections)} axes")
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * sum(sections) > d:
+        raise ValueError(f"{what}: sections {sections} of a head of {d} channels (1 to 4 axes, at most {d // 2} pairs)")
+    if not 1.0 < float(base) < 1e30:
+        raise ValueError(f"{what}: base {base}")
+    positions = positions.contiguous()
+    posb = N * len(sections) if positions.dim() == 3 and positions.shape[0] == B else 0
+    return positions, (_POS_KIND[positions.dtype], posb, len(sections), *sections, *(0,) * (4 - len(sections)), float(base), int(bool(interleaved)))
+
+
+def _norm_weights(what, d, *ws):
+    out = []
+    for w in ws:
+        if w.dtype != torch.float32 or tuple(w.shape) != (d,):
+            raise ValueError(f"{what}: the norm's weights and biases are float32 [{d}], got {w.dtype} {tuple(w.shape)}")
+        w = w.detach().contiguous()
+        out.append(w if w.data_ptr() % 16 == 0 else w.clone())
+    return out
+
+
+class RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, heads, positions, rot):
+        xs, (xb, xt) = _strided(x)
+        B, N, W = x.shape
+        y = torch.empty((B, N, W), dtype=x.dtype, device=x.device)
+        with _device_of(x):
+            _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, 0, W // heads, 0, 0, 0, 0, 0.0, _p(positions), *rot, 0,
+                      _dt(x), _stream())
+        ctx.save_for_backward(positions)
+        ctx.heads, ctx.rot = heads, rot
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        (positions,) = ctx.saved_tensors
+        gs, (gb, gt) = _strided(g)
+        B, N, W = g.shape
+        gx = torch.empty((B, N, W), dtype=g.dtype, device=g.device)
+        with _device_of(g):
+            _lib.call("dp_qk_rotary_fwd", _p(gs), gb, gt, _p(gx), N * W, W, B, N, ctx.heads, 0, W // ctx.heads, 0, 0, 0, 0, 0.0, _p(positions),
+                      *ctx.rot, 1, _dt(g), _stream())
+        return gx, None, None, None
+
+
+def rotary_axes(x, heads, positions, sections, base=10000.0, interleaved=False):
+    """Rotary positions over the axes of a token grid: x [B, N, heads * d] (rows may be slices of wider ones) with every pair of a head turned
+    by its token's angle.  positions [N, axes] or [B, N, axes] (int32, int64 or float32); sections: rotated pairs of a head per axis -- pair e
+    of an axis with n pairs turns by position * base^(-e / n); pairs behind the sections stay.  interleaved False: pair i = channels
+    (i, i + d / 2), True: (2 i, 2 i + 1).  d in HEAD_DIMS.  The gradient is the turn backwards; positions have none."""
+    _dt(x)
+    if x.dim() != 3:
+        raise ValueError(f"rotary_axes: x is [B, N, channels], got {tuple(x.shape)}")
+    d = _head_dim(x.shape[-1], heads, "rotary_axes")
+    positions, rot = _rotary_args("rotary_axes", x, d, positions, sections, base, interleaved)
+    _chk_dev(x)
+    return RotaryAxes.apply(x, int(heads), positions, rot)
+
+
+class QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, qw, qb, kw, kb, heads, kv, eps, positions, rot):
+        xs, (xb, xt) = _strided(x)
+        B, N, W = x.shape
+        d = W // (heads + kv)
+        qwd, qbd, kwd, kbd = _norm_weights("qk_norm_rotary", d, qw, qb, kw, kb)
+        y = torch.empty((B, N, W), dtype=x.dtype, device=x.device)
+        with _device_of(x):
+            _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, kv, d, _p(qwd), _p(qbd), _p(kwd), _p(kbd), eps,
+                      _p(positions), *rot, 0, _dt(x), _stream())
+        ctx.save_for_backward(xs, qw, kw, positions)
+        ctx.opts = (xb, xt, heads, kv, eps, rot)
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        xs, qw, kw, positions = ctx.saved_tensors
+        xb, xt, heads, kv, eps, rot = ctx.opts
+        gs, (gb, gt) = _strided(g)
+        B, N, W = g.shape
+        d = W // (heads + kv)
+        qwd, kwd = _norm_weights("qk_norm_rotary", d, qw, kw)
+        gx = torch.empty((B, N, W), dtype=g.dtype, device=g.device)
+        dw = torch.empty((4, d), dtype=torch.float32, device=g.device)
+        part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=g.device)
+        with _device_of(g):
+            _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(gs), gb, gt, 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d, _p(qwd),
+                      _p(kwd), eps, _p(positions), *rot, _dt(g), _stream())
+        return gx, dw[0], dw[1], dw[2], dw[3], None, None, None, None, None
+
+
+def qk_norm_rotary(x, heads, kv_heads, q_weight, q_bias, k_weight, k_bias, eps=1e-5, positions=None, sections=None, base=10000.0,
+                   interleaved=False):
+    """LayerNorm of every head of queries and keys -- x [B, N, (heads + kv_heads) * d], rows may be slices of wider ones; one float32 [d]
+    weight and bias for all query heads, one for all key heads -- and, with positions, the rotation of rotary_axes behind it, in one pass.
+    The weights' gradients are added up in a fixed order."""
+    what = "qk_norm_rotary"
+    _dt(x)
+    if x.dim() != 3 or heads < 1 or kv_heads < 1:
+        raise ValueError(f"{what}: x is [B, N, channels] with heads and kv_heads of at least 1, got {tuple(x.shape)}, {heads}, {kv_heads}")
+    d = _head_dim(x.shape[-1], heads + kv_heads, what)
+    _norm_weights(what, d, q_weight, q_bias, k_weight, k_bias)
+    positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
+    _chk_dev(x, q_weight, q_bias, k_weight, k_bias)
+    return QkNormRotary.apply(x, q_weight, q_bias, k_weight, k_bias, int(heads), int(kv_heads), float(eps), positions, rot)
+
+
+# ------------------------------------------------------------------------------------------------ attention over a sliding window
+def _per_sequence(what, name, t, B, like):
+    """int32 [B] on the rows' device."""
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,):
+        raise ValueError(f"{what}: {name} is int32 or int64 [{B}], got {t.dtype} {tuple(t.shape)}")
+    if t.device != like.device:
+        raise _lib.DoseHipError(f"{what}: {name} on {t.device}, rows on {like.device}")
+    return t.to(torch.int32).contiguous()
+
+
+def _window_args(what, left, right, sinks, scale, d):
+    for name, v in (("left", left), ("right", right)):
+        if v is not None and not 0 <= int(v) < 1 << 31:
+            raise ValueError(f"{what}: {name} is None or at least 0, got {v}")
+    left, right = (-1 if v is None else int(v) for v in (left, right))
+    sinks = int(sinks)
+    if not 0 <= sinks < 1 << 31:
+        raise ValueError(f"{what}: sinks {sinks}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"{what}: scale {scale}")
+    return left, right, sinks, scale
+
+
+def _window_ws(B, heads, kv, Nq, Nk, d, win, backward, dev):
+    n = _lib.lib().dp_window_attention_ws_elems(B, heads, kv, Nq, Nk, d, win[0], win[1], win[2], backward)
+    return torch.empty((n,), dtype=torch.float32, device=dev) if n else None
+
+
+class WindowAttention(torch.autograd.Function):
+    """q [B, Nq, heads, d], k / v [B, Nk, kv, d]; win = (left, right, sinks, scale)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, win, start, starts, lengths):
+        (qs, qst), (ks, kst), (vs, vst) = _strided(q), _strided(k), _strided(v)
+        (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
+        o = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
+        need = any(ctx.needs_input_grad[:3])
+        lse = torch.empty((B * heads * Nq,), dtype=torch.float32, device=q.device) if need else None
+        with _device_of(q):
+            ws = _window_ws(B, heads, kv, Nq, Nk, d, win, 0, q.device)
+            _lib.call("dp_window_attention_fwd", _p(qs), *qst, _p(ks), *kst, _p(vs), *vst, _p(o), Nq * heads * d, heads * d, d, _p(lse), _p(ws),
+                      B, heads, kv, Nq, Nk, d, win[0], win[1], win[2], start, _p(starts), _p(lengths), win[3], _dt(q), _stream())
+        if need:
+            ctx.save_for_backward(qs, ks, vs, o, lse, starts, lengths)
+            ctx.opts = (qst, kst, vst, win, start)
+        return o
+
+    @staticmethod
+    def backward(ctx, g):
+        q, k, v, o, lse, starts, lengths = ctx.saved_tensors
+        qst, kst, vst, win, start = ctx.opts
+        gs, gst = _strided(g)
+        (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
+        dq = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
+        dk = torch.empty((B, Nk, kv, d), dtype=q.dtype, device=q.device)
+        dv = torch.empty_like(dk)
+        delta = torch.empty_like(lse)
+        with _device_of(q):
+            ws = _window_ws(B, heads, kv, Nq, Nk, d, win, 1, q.device)
+            _lib.call("dp_window_attention_bwd", _p(q), *qst, _p(k), *kst, _p(v), *vst, _p(o), Nq * heads * d, heads * d, d, _p(gs), *gst, _p(lse),
+                      _p(delta), _p(dq), Nq * heads * d, heads * d, d, _p(dk), Nk * kv * d, kv * d, d, _p(dv), Nk * kv * d, kv * d, d, 0, _p(ws), B,
+                      heads, kv, Nq, Nk, d, win[0], win[1], win[2], start, _p(starts), _p(lengths), win[3], _dt(q), _stream())
+        return dq, dk, dv, None, None, None, None
+
+
+def window_attention(q, k, v, left=None, right=None, sinks=0, q_start=0, lengths=None, scale=None):
+    """softmax(scale q k^T) v over a sliding window, whose first tokens stay visible.  q [B, Nq, heads, d], k and v [B, Nk, kv_heads, d] (any
+    strides; heads % kv_heads == 0: that many query heads share a key head; d in HEAD_DIMS); returns [B, Nq, heads, d].
+
+    The query in row i stands at position p = q_start + i (q_start: an int, or int32 / int64 [B]) and sees key j iff j < lengths[b],
+    j <= p + right, and j >= p - left or j < sinks.  left / right None: no limit on that side; right=0 looks back only.  lengths (int32 /
+    int64 [B], None: all Nk keys): rows at positions outside [0, lengths[b]) give 0 and get and cause no gradient, whatever they hold, NaN
+    included.  (A value that is not finite inside a sequence reaches the rows it is seen by, and may reach others near them.)
+    scale None: d^-1/2.  Sums are added in a fixed order: the same inputs give the same bits."""
+    what = "window_attention"
+    _dt(q)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{what}: q [B, Nq, heads, d], k and v [B, Nk, kv_heads, d], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+        raise TypeError(f"{what}: q, k and v share type and device, got {q.dtype}, {k.dtype}, {v.dtype} on {q.device}, {k.device}, {v.device}")
+    B, heads, kv, d = q.shape[0], q.shape[2], k.shape[2], q.shape[3]
+    if heads < 1 or kv < 1 or heads % kv:
+        raise ValueError(f"{what}: {heads} query heads do not divide over {kv} key heads")
+    _head_dim(heads * d, heads, what)
+    win = _window_args(what, left, right, sinks, scale, d)
+    starts = None
+    if torch.is_tensor(q_start):
+        starts, q_start = _per_sequence(what, "q_start", q_start, B, q), 0
+    if abs(int(q_start)) >= 1 << 30:
+        raise ValueError(f"{what}: q_start {q_start}")
+    lengths = _per_sequence(what, "lengths", lengths, B, q)
+    _chk_dev(q)
+    return WindowAttention.apply(q, k, v, win, int(q_start), starts, lengths)
+
+
+class WindowAttentionQkv(torch.autograd.Function):
+    """The packed projection's form: norm and rotation of q and k into a buffer of their own (one launch, none without them), v read in
+    place; the backward pass writes one packed gradient, that of q and k passing through the norm and the rotation unrounded (float)."""
+
+    @staticmethod
+    def forward(ctx, qkv, qw, qb, kw, kb, heads, kv, eps, positions, rot, win, lengths):
+        xs, (xb, xt) = _strided(qkv)
+        B, N, W = qkv.shape
+        d, es, dtc = W // (heads + 2 * kv), qkv.element_size(), _dt(qkv)
+        Wq, Wqk = heads * d, (heads + kv) * d
+        pre = qw is not None or positions is not None
+        o = torch.empty((B, N, Wq), dtype=qkv.dtype, device=qkv.device)
+        need = any(ctx.needs_input_grad[:5])
+        lse = torch.empty((B * heads * N,), dtype=torch.float32, device=qkv.device) if need else None
+        with _device_of(qkv):
+            qk, qkb, qkt = xs, xb, xt
+            if pre:
+                ws4 = _norm_weights("window_attention_qkv", d, qw, qb, kw, kb) if qw is not None else (None,) * 4
+                qk, qkb, qkt = torch.empty((B, N, Wqk), dtype=qkv.dtype, device=qkv.device), N * Wqk, Wqk
+                _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(qk), qkb, qkt, B, N, heads, kv, d, *(_p(w) for w in ws4), eps, _p(positions), *rot,
+                          0, dtc, _stream())
+            ws = _window_ws(B, heads, kv, N, N, d, win, 0, qkv.device)
+            _lib.call("dp_window_attention_fwd", _p(qk), qkb, qkt, d, _p(qk) + Wq * es, qkb, qkt, d, _p(xs) + Wqk * es, xb, xt, d, _p(o), N * Wq, Wq, d,
+                      _p(lse), _p(ws), B, heads, kv, N, N, d, win[0], win[1], win[2], 0, 0, _p(lengths), win[3], dtc, _stream())
+        if need:
+            ctx.save_for_backward(xs, qk if pre else None, o, lse, qw, kw, positions, lengths)
+            ctx.opts = (xb, xt, heads, kv, eps, rot, win)
+        return o
+
+    @staticmethod
+    def backward(ctx, g):
+        xs, qk, o, lse, qw, kw, positions, lengths = ctx.saved_tensors
+        xb, xt, heads, kv, eps, rot, win = ctx.opts
+        gs, (gb, gt) = _strided(g)
+        B, N, W = xs.shape
+        d, es, dtc, dev = W // (heads + 2 * kv), xs.element_size(), _dt(xs), xs.device
+        Wq, Wqk = heads * d, (heads + kv) * d
+        gx = torch.empty((B, N, W), dtype=xs.dtype, device=dev)
+        delta = torch.empty_like(lse)
+        dw = None
+        with _device_of(xs):
+            ws = _window_ws(B, heads, kv, N, N, d, win, 1, dev)
+            src, sb, stt = (xs, xb, xt) if qk is None else (qk, N * Wqk, Wqk)
+            # dq, dk: into the packed gradient, or (16-bit storage, norm / rotation still to come) into a float buffer
+            wide = qk is not None and xs.dtype != torch.float32
+            dst, db, dt_, des = (torch.empty((B, N, Wqk), dtype=torch.float32, device=dev), N * Wqk, Wqk, 4) if wide else (gx, N * W, W, es)
+            _lib.call("dp_window_attention_bwd", _p(src), sb, stt, d, _p(src) + Wq * es, sb, stt, d, _p(xs) + Wqk * es, xb, xt, d, _p(o), N * Wq, Wq, d,
+                      _p(gs), gb, gt, d, _p(lse), _p(delta), _p(dst), db, dt_, d, _p(dst) + Wq * des, db, dt_, d, _p(gx) + Wqk * es, N * W, W, d,
+                      1 if wide else 0, _p(ws), B, heads, kv, N, N, d, win[0], win[1], win[2], 0, 0, _p(lengths), win[3], dtc, _stream())
+            if qk is not None:
+                part = None
+                if qw is not None:
+                    qw, kw = _norm_weights("window_attention_qkv", d, qw, kw)
+                    dw = torch.empty((4, d), dtype=torch.float32, device=dev)
+                    part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=dev)
+                _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d,
+                          _p(qw), _p(kw), eps, _p(positions), *rot, dtc, _stream())
+        return (gx, *((dw[0], dw[1], dw[2], dw[3]) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
+
+
+def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks=0, lengths=None, scale=None, norm=None, eps=1e-5,
+                         positions=None, sections=None, base=10000.0, interleaved=False):
+    """The attention block's core on the packed projection [B, N, (heads + 2 kv_heads) * d] ("q heads | k heads | v heads", kv_heads None:
+    as many as heads), as attention() takes it: with norm = (q_weight, q_bias, k_weight, k_bias) the LayerNorm of qk_norm_rotary, with
+    positions the rotation of rotary_axes, then window_attention of the rows with themselves.  Returns [B, N, heads * d]."""
+    what = "window_attention_qkv"
+    norm = tuple(norm) if norm is not None else (None,) * 4
+    if len(norm) != 4:
+        raise ValueError(f"{what}: norm is (q_weight, q_bias, k_weight, k_bias)")
+    _dt(qkv)
+    kv = int(heads if kv_heads is None else kv_heads)
+    if qkv.dim() != 3 or heads < 1 or kv < 1 or heads % kv:
+        raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
+    d = _head_dim(qkv.shape[-1], heads + 2 * kv, what)
+    if norm[0] is not None:
+        _norm_weights(what, d, *norm)
+    positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
+    win = _window_args(what, left, right, sinks, scale, d)
+    lengths = _per_sequence(what, "lengths", lengths, qkv.shape[0], qkv)
+    _chk_dev(qkv, *norm)
+    return WindowAttentionQkv.apply(qkv, *norm, int(heads), kv, float(eps), positions, rot, win, lengths)
+
+
 # ------------------------------------------------------------------------------------------------ misc
 class Patchify(torch.autograd.Function):
     """einops "b c (h p1)(w p2)(d p3) -> b (h w d)(p1 p2 p3 c)" on an NDHWC tensor (first C channels)."""

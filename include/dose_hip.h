@@ -204,6 +204,52 @@ int dp_add_layernorm_bwd_det(const void* x, const void* gy, const void* gsum, co
                              void* gx, float* part, float* dgamma, float* dbeta, int64_t rows, int C, int dtype, void* stream);
 
 
+/* ---- rotary positions and the norm of queries and keys (beside MONAI's learned position embedding, dose_pyfer.py:55-67) ----------------
+ * Rows [B][N] of heads + kv_heads heads of d channels, d in {32, 64, 96, 128}, heads beside each other: head h of token t of sequence b
+ * starts at x + b * xb + t * xt + h * d (element strides; every row 16-byte aligned).  The first `heads` heads are queries, the next
+ * kv_heads keys.
+ *   norm (weights not NULL): u = LayerNorm over the d channels of each head, weight / bias fp32 [d] shared by the heads (wq, bq for
+ *     queries, wk, bk for keys; a group without heads needs none);
+ *   rotation (pos not NULL): pair i of a head is turned by position[t][axis(i)] * base^(-e / pairs(axis)): the first s0 pairs belong to
+ *     axis 0 with e = 0 .. s0 - 1, the next s1 to axis 1 and so on (naxes <= 4, s0 + s1 + s2 + s3 <= d / 2; pairs behind them stay as they
+ *     are).  interleaved 0: pair i = channels (i, i + d / 2); 1: channels (2 i, 2 i + 1).  pos: contiguous [B][N][naxes] with posb elements
+ *     between sequences (0: one table [N][naxes] for all); pos_kind 0 int32, 1 int64, 2 float.  Angles are formed in 64 bits.
+ *   inverse != 0 turns back (the gradient of the rotation alone).  y may be x.
+ * dp_qk_rotary_bwd: gx from gy (g_f32 != 0: gy is float whatever the storage type; gx may be gy where the types agree); with a norm also
+ * dw[4][d] = gradients of wq, bq, wk, bk (OVERWRITTEN; those of a group without heads are zero), from part, a scratch of
+ * dp_qk_rotary_parts(B * N) x 4 x d floats, added in a fixed order.  Without a norm x, part and dw may be NULL. */
+int dp_qk_rotary_parts(int64_t tokens);
+int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, int64_t yb, int64_t yt, int B, int64_t N, int heads, int kv_heads, int d,
+                     const float* wq, const float* bq, const float* wk, const float* bk, float eps, const void* pos, int pos_kind, int64_t posb,
+                     int naxes, int s0, int s1, int s2, int s3, double base, int interleaved, int inverse, int dtype, void* stream);
+int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const void* g, int64_t gb, int64_t gt, int g_f32, void* gx, int64_t gxb, int64_t gxt,
+                     float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
+                     const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
+                     int dtype, void* stream);
+
+/* ---- attention over a sliding window whose first tokens stay visible (beside dp_attention_*, for token rows too long for it) ------------
+ * q, o, go, dq: [B][Nq][heads][d], k, v, dk, dv: [B][Nk][kv_heads][d], each with its own element strides of sequence, token and head (rows
+ * dense and 16-byte aligned); heads % kv_heads == 0, query heads kv * group .. + group - 1 share key head kv; d in {32, 64, 96, 128};
+ * dtype DP_F32, DP_BF16 or DP_F16 (fp32: exact fp32 MFMA chain), accumulation and softmax statistics fp32.
+ * The query in row i stands at p = start + i, start = q_starts[b] (device int32, or NULL: q_start); n = lengths[b] (device int32, clamped
+ * to [0, Nk]; NULL: Nk).  It sees key j iff p in [0, n), j < n, j <= p + right and (j >= p - left or j < sinks); left / right -1: no limit.
+ * Rows that see nothing give 0; rows and keys outside the sequence are never read into a result.  scale > 0.
+ * fwd: lse float [B * kv_heads][Nq * group] (base-2 log-sum-exp of the scaled scores, row = i * group + head in group, +inf for empty
+ * rows; NULL: not wanted).  bwd: delta float of the same size (scratch); dq, dk, dv are OVERWRITTEN (zeros outside the sequence);
+ * qk_f32 != 0: dq and dk are float whatever the storage type.  ws: dp_window_attention_ws_elems(..., backward) floats, 16-byte aligned
+ * (NULL when that is 0).  No atomics: the same inputs give the same bits. */
+int64_t dp_window_attention_ws_elems(int B, int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int backward);
+int dp_window_attention_fwd(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* k, int64_t kb, int64_t kt, int64_t kh, const void* v,
+                            int64_t vb, int64_t vt, int64_t vh, void* o, int64_t ob, int64_t ot, int64_t oh, float* lse, float* ws, int B,
+                            int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int q_start, const int32_t* q_starts,
+                            const int32_t* lengths, float scale, int dtype, void* stream);
+int dp_window_attention_bwd(const void* q, int64_t qb, int64_t qt, int64_t qh, const void* k, int64_t kb, int64_t kt, int64_t kh, const void* v,
+                            int64_t vb, int64_t vt, int64_t vh, const void* o, int64_t ob, int64_t ot, int64_t oh, const void* go, int64_t gb,
+                            int64_t gt, int64_t gh, const float* lse, float* delta, void* dq, int64_t dqb, int64_t dqt, int64_t dqh, void* dk,
+                            int64_t dkb, int64_t dkt, int64_t dkh, void* dv, int64_t dvb, int64_t dvt, int64_t dvh, int qk_f32, float* ws, int B,
+                            int heads, int kv_heads, int Nq, int Nk, int d, int left, int right, int sinks, int q_start, const int32_t* q_starts,
+                            const int32_t* lengths, float scale, int dtype, void* stream);
+
 /* ---- matrix products (MFMA) ------------------------------------------------------------------- */
 /* C[b0][b1][m][n] = alpha * sum_k A[..][m][k] * B[..][n][k] (+ bias[n]) ; "NT" GEMM, both operands k-contiguous.
  * replaces: nn.Linear (MONAI ViT), 1x1x1 nn.Conv3d (blocks_MDUNet.py:146, dose_pyfer.py:292,353), the GEMM half of
