@@ -37,16 +37,16 @@ __device__ __forceinline__ v16f zero16() { v16f z; for (int i = 0; i < 16; i++) 
 
 template <typename T> __device__ __forceinline__ Frag8<T> ldg8(const T* p) { Frag8<T> f; f.u = *(const v4u*)p; return f; }
 template <> __device__ __forceinline__ Frag8<float> ldg8<float>(const float* p) { return frag_ld_lds(p); }
-__device__ __forceinline__ Frag8<bf16_t> pack8(const float* p, bf16_t) {
-  Frag8<bf16_t> f;
+// (pairs through vector conversions: one v_cvt_pk per two values)
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned pack_pair(float a, float b, bf16_t) { return __builtin_bit_cast(unsigned, __builtin_convertvector((v2f){a, b}, v2bf)); }
+__device__ __forceinline__ unsigned pack_pair(float a, float b, f16_t) { return __builtin_bit_cast(unsigned, __builtin_convertvector((v2f){a, b}, v2h)); }
+template <typename T> __device__ __forceinline__ Frag8<T> pack8(const float* p, T t) {
+  Frag8<T> f;
 #pragma unroll
-  for (int i = 0; i < 4; i++) f.u[i] = (unsigned)f2bf(p[2 * i]) | ((unsigned)f2bf(p[2 * i + 1]) << 16);
-  return f;
-}
-__device__ __forceinline__ Frag8<f16_t> pack8(const float* p, f16_t) {
-  Frag8<f16_t> f;
-#pragma unroll
-  for (int i = 0; i < 4; i++) f.u[i] = (unsigned)__builtin_bit_cast(unsigned short, (f16_t)p[2 * i]) | ((unsigned)__builtin_bit_cast(unsigned short, (f16_t)p[2 * i + 1]) << 16);
+  for (int i = 0; i < 4; i++) f.u[i] = pack_pair(p[2 * i], p[2 * i + 1], t);
   return f;
 }
 __device__ __forceinline__ Frag8<float> pack8(const float* p, float) {
@@ -61,12 +61,16 @@ template <typename T> __device__ __forceinline__ float elem(const Frag8<T>& f, i
 }
 template <> __device__ __forceinline__ float elem<float>(const Frag8<float>& f, int i) { return f.v[i]; }
 __device__ __forceinline__ void st4(float* p, const float* v) { *(v4f*)p = (v4f){v[0], v[1], v[2], v[3]}; }
-__device__ __forceinline__ void st4(bf16_t* p, const float* v) {
-  *(uint2*)p = make_uint2((unsigned)f2bf(v[0]) | ((unsigned)f2bf(v[1]) << 16), (unsigned)f2bf(v[2]) | ((unsigned)f2bf(v[3]) << 16));
+template <typename T> __device__ __forceinline__ void st4(T* p, const float* v) { *(uint2*)p = make_uint2(pack_pair(v[0], v[1], T{}), pack_pair(v[2], v[3], T{})); }
+
+// over the two lanes that hold halves of one owned row
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ void st4(f16_t* p, const float* v) {
-  typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-  *(v4h*)p = (v4h){(f16_t)v[0], (f16_t)v[1], (f16_t)v[2], (f16_t)v[3]};
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 template <typename T, int D> struct Cfg {
@@ -93,6 +97,11 @@ template <typename T, int D> __device__ __forceinline__ Frag8<T> tr_frag(const T
 TR_F32(32) TR_F32(64) TR_F32(96) TR_F32(128)
 #undef TR_F32
 
+// Waves per SIMD that the register budget is cut for.  Two (256 registers) also keep the matrix accumulators in plain VGPRs: with more the
+// compiler puts them into AGPRs and copies them back and forth around every rescale and mask (24 instead of 9 vector instructions per
+// matrix instruction in the forward kernel).  One where two would spill.
+template <typename T, int D> constexpr int waves_q() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
+template <typename T, int D> constexpr int waves_kv() { return D == 128 || (sizeof(T) == 4 && D >= 64) ? 1 : 2; }
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
   Mat q, k, v, o, go, dq, dk, dv;
@@ -200,9 +209,26 @@ __device__ __forceinline__ Row row_of(const WinArgs& a, const Seq& s, int r) {
   return w;
 }
 
+// scores of keys k0 .. k0 + 31 that the lane's row does not see -> `none`.  Behind the sinks a seen key is one range: one subtraction and one
+// unsigned comparison a key.  (A row that is not live may keep any value: its column is thrown away.)
+__device__ __forceinline__ void mask_keys(v16f& s, const Row& row, int k0, int h, int sinks, float none) {
+  if (k0 < sinks) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int j = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+      s[i] = (j <= row.hi && (j >= row.lo || j < sinks)) ? s[i] : none;
+    }
+    return;
+  }
+  const int off = k0 + 4 * h - row.lo;
+  const unsigned span = (unsigned)(row.hi - row.lo);
+#pragma unroll
+  for (int i = 0; i < 16; i++) s[i] = (unsigned)(off + 8 * (i >> 2) + (i & 3)) <= span ? s[i] : none;
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256) void k_win_fwd(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -243,19 +269,14 @@ __global__ __launch_bounds__(256) void k_win_fwd(const WinArgs a) {
     }
     if (!all) {
 #pragma unroll
-      for (int u = 0; u < S::KS; u++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int j = k0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-          s[u][i] = (j <= row.hi && (j >= row.lo || j < a.sinks)) ? s[u][i] : -INFINITY;
-        }
+      for (int u = 0; u < S::KS; u++) mask_keys(s[u], row, k0 + 32 * u, h, a.sinks, -INFINITY);
     }
     float mx = s[0][0];
 #pragma unroll
     for (int u = 0; u < S::KS; u++)
 #pragma unroll
       for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = pair_max(mx);
     const float mn = fmaxf(m, mx);
     if (__builtin_amdgcn_ballot_w64(mn > m)) {        // (the maximum of a row moves in its first tiles, hardly ever after them)
       // (alpha from the rounded products: exactly 1 for the rows whose maximum stays, whatever the wave's other rows hold)
@@ -295,7 +316,7 @@ __global__ __launch_bounds__(256) void k_win_fwd(const WinArgs a) {
       lds_barrier();
       buf ^= 1;
     }
-    l += __shfl_xor(l, 32, 64);
+    l = pair_sum(l);
     if (row.r < a.rows) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* Or = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)row.i * a.o.t + (int64_t)(kvh * a.group + row.g) * a.o.h;
@@ -324,7 +345,7 @@ __global__ __launch_bounds__(256) void k_win_fwd(const WinArgs a) {
     compute(ks, vs, key_of(t));
     wave_lds_sync();
   }
-  l += __shfl_xor(l, 32, 64);
+  l = pair_sum(l);
   if (!row.live) { l = 0.f; m = -INFINITY; }
   float* part = (float*)smem;
   float* mw = (float*)(smem + S::big);
@@ -403,7 +424,7 @@ template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t 
 
 // ------------------------------------------------------------------------------------------------ backward: dQ (and delta)
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256) void k_win_dq(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -428,7 +449,7 @@ __global__ __launch_bounds__(256) void k_win_dq(const WinArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; i++) dl += elem(of, i) * elem(gf[kk], i);
   }
-  dl += __shfl_xor(dl, 32, 64);
+  dl = pair_sum(dl);
   const float lse = row.live ? a.lse[(int64_t)bh * a.rows + row.r] : INFINITY;
   if (row.r < a.rows && h == 0 && (WIDE || wv == 0)) a.delta[(int64_t)bh * a.rows + row.r] = row.live ? dl : 0.f;
   const float ds0 = -dl * a.scale;
@@ -454,13 +475,7 @@ __global__ __launch_bounds__(256) void k_win_dq(const WinArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, ds0);
-      if (!all) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int j = k0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-          s[i] = (j <= row.hi && (j >= row.lo || j < a.sinks)) ? s[i] : 0.f;
-        }
-      }
+      if (!all) mask_keys(s, row, k0 + 32 * u, h, a.sinks, 0.f);
 #pragma unroll
       for (int st = 0; st < 2; st++) {
         float p[8];
@@ -553,7 +568,7 @@ __device__ __forceinline__ Span rows_of(const WinArgs& a, const Seq& s, int jlo,
 }
 
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256) void k_win_dkv(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -581,10 +596,10 @@ __global__ __launch_bounds__(256) void k_win_dkv(const WinArgs a) {
   v16f ak[C::DT], av[C::DT];
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++) { ak[dt] = zero16(); av[dt] = zero16(); }
-  const Span mine = live ? rows_of(a, sq, j, j) : Span{0x7fffffff, 0};
+  const Span mine = live ? rows_of(a, sq, j, j) : Span{0x7fffffff, 0x7fffffff};
   const Span block = k0 < sq.len ? rows_of(a, sq, k0, min(k0 + S::ROWS, sq.len) - 1) : Span{0, 0};
   // (rows that all keys of the wave see need no mask, rows that none of them sees no work)
-  int all_lo = mine.lo, all_hi = mine.hi, any_lo = mine.lo, any_hi = mine.hi;
+  int all_lo = mine.lo, all_hi = live ? mine.hi : 0, any_lo = mine.lo, any_hi = live ? mine.hi : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     all_lo = max(all_lo, __shfl_xor(all_lo, o, 64)); all_hi = min(all_hi, __shfl_xor(all_hi, o, 64));
@@ -614,8 +629,7 @@ __global__ __launch_bounds__(256) void k_win_dkv(const WinArgs a) {
         for (int i = 0; i < 4; i++) {
           float p = __builtin_amdgcn_exp2f(fmaf(s[4 * q + i], a.c, -ls[i])), d = p * fmaf(dp[4 * q + i], a.scale, -dl[i]);
           if (!all) {
-            const int r = r0 + 8 * q + 4 * h + i;
-            const bool see = r >= mine.lo && r < mine.hi;
+            const bool see = (unsigned)(r0 + 8 * q + 4 * h + i - mine.lo) < (unsigned)(mine.hi - mine.lo);
             p = see ? p : 0.f; d = see ? d : 0.f;
           }
           s[4 * q + i] = p; dp[4 * q + i] = d;
