@@ -248,19 +248,27 @@ __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const Rot
   }
 }
 
-// dw[i] = sum over the partial rows, in a fixed order: 16 row strips per column, each added in 64 bits
+// dw[i] = sum over the partial rows, in a fixed order: 32 row strips per column, each added in 64 bits with four loads in flight
 __global__ void __launch_bounds__(1024) k_qk_dw_sum(const float* __restrict__ part, float* __restrict__ dw, int rows, int cols) {
-  __shared__ double red[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), strip = threadIdx.x >> 6;
+  __shared__ double red[32][32];
+  const int cc = threadIdx.x & 31, col = blockIdx.x * 32 + cc, strip = threadIdx.x >> 5;
   double s = 0.0;
-  if (col < cols)
-    for (int r = strip; r < rows; r += 16) s += (double)part[(int64_t)r * cols + col];
-  red[strip][threadIdx.x & 63] = s;
+  if (col < cols) {
+    int r = strip;
+    for (; r + 96 < rows; r += 128) {
+      const float* p = part + (int64_t)r * cols + col;
+      const float x0 = p[0], x1 = p[32 * cols], x2 = p[64 * cols], x3 = p[96 * cols];
+      s += ((double)x0 + (double)x1) + ((double)x2 + (double)x3);
+    }
+    for (; r < rows; r += 32) s += (double)part[(int64_t)r * cols + col];
+  }
+  red[strip][cc] = s;
   __syncthreads();
   if (strip == 0 && col < cols) {
+    double t[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int k = 1; k < 16; k++) s += red[k][threadIdx.x];
-    dw[col] = (float)s;
+    for (int k = 0; k < 32; k++) t[k & 3] += red[k][cc];
+    dw[col] = (float)((t[0] + t[1]) + (t[2] + t[3]));
   }
 }
 
@@ -340,7 +348,7 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
   if (make_plan("qk_rotary_bwd", R, pos, pos_kind, posb, naxes, sec, base, interleaved, d)) return 1;
   const int64_t tokens = (int64_t)B * N;
   if (tokens == 0 || heads + kv_heads == 0) {
-    if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 64)), dim3(1024), 0, STREAM, (const float*)part, dw, 0, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd"); }
+    if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 32)), dim3(1024), 0, STREAM, (const float*)part, dw, 0, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd"); }
     return 0;
   }
   const int tok = block_tokens(tokens);
@@ -352,6 +360,6 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
                                                  else hipLaunchKernelGGL((k_qk_rotary_bwd<T, TG, D, false>), dim3(nblk), dim3(256), smem, STREAM, a, R)))
   if (g_f32) QK_BWD(float); else QK_BWD(T);
   DP_CHECK_LAUNCH("qk_rotary_bwd");
-  if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 64)), dim3(1024), 0, STREAM, (const float*)part, dw, nblk, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd(dw)"); }
+  if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 32)), dim3(1024), 0, STREAM, (const float*)part, dw, nblk, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd(dw)"); }
   return 0;
 }

@@ -101,7 +101,7 @@ TR_F32(32) TR_F32(64) TR_F32(96) TR_F32(128)
 // compiler puts them into AGPRs and copies them back and forth around every rescale and mask (24 instead of 9 vector instructions per
 // matrix instruction in the forward kernel).  One where two would spill.
 template <typename T, int D> constexpr int waves_q() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
-template <typename T, int D> constexpr int waves_kv() { return D == 128 || (sizeof(T) == 4 && D >= 64) ? 1 : 2; }
+template <typename T, int D> constexpr int waves_kv() { return D >= 96 || (sizeof(T) == 4 && D >= 64) ? 1 : 2; }
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
   Mat q, k, v, o, go, dq, dk, dv;
@@ -171,6 +171,8 @@ template <typename T, int D, bool WIDE> struct Shape {
   // WIDE: four waves own 32 rows each and share every staged tile (two LDS buffers, one barrier per tile).  Otherwise all four own the same
   // 32 rows, stream different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
   static constexpr int KS = (WIDE && C::ES == 2) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64, NBUF = WIDE ? 2 : 1;
+  // the next tile waits in registers while this one is worked on: not in the narrow fp32 kernels, where it would spill (a wave has few tiles)
+  static constexpr bool AHEAD = WIDE || C::ES == 2;
   static constexpr size_t tile = (size_t)KT * C::LDP * C::ES;
   static constexpr size_t stage = WIDE ? 2 * NBUF * tile : 4 * 2 * tile;
   static constexpr size_t merge = WIDE ? 0 : (size_t)4 * 32 * C::CP * 4;
@@ -207,6 +209,28 @@ __device__ __forceinline__ Row row_of(const WinArgs& a, const Seq& s, int r) {
   w.hi = w.live ? min(w.p + a.right, s.len - 1) : -1;
   w.lo = w.live ? w.p - a.left : 0;
   return w;
+}
+
+// The LDS reads written above this line are issued before what follows: left alone, the compiler reads each operand right in front of its
+// matrix instruction and waits out the LDS latency every time.
+// (fp32 operands take twice the registers: there the compiler's own order stays)
+#define READS_FIRST do { if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0); } while (0)
+// Loads of the prologue are waited for here: otherwise the waits for them sit inside the loop, where they hold up the prefetch instead.
+#define PROLOGUE_LOADED __builtin_amdgcn_s_waitcnt(0)
+
+// s += X x, t += Y y over the head dimension: rows of two staged tiles (x0, y0: the lane's first piece) against fragments in registers
+template <typename T, int D>
+__device__ __forceinline__ void two_products(const T* x0, const T* y0, const Frag8<T>* x, const Frag8<T>* y, v16f& s, v16f& t) {
+  constexpr int KK = Cfg<T, D>::KK, G = sizeof(T) == 4 ? 1 : KK < 4 ? KK : KK == 6 ? 3 : 4;      // (an fp32 operand is twice the registers)
+#pragma unroll
+  for (int g = 0; g < KK; g += G) {
+    Frag8<T> xf[G], yf[G];
+#pragma unroll
+    for (int i = 0; i < G; i++) { xf[i] = frag_ld_lds(x0 + 16 * (g + i)); yf[i] = frag_ld_lds(y0 + 16 * (g + i)); }
+    READS_FIRST;
+#pragma unroll
+    for (int i = 0; i < G; i++) { s = mma32(xf[i], x[g + i], s); t = mma32(yf[i], y[g + i], t); }
+  }
 }
 
 // scores of keys k0 .. k0 + 31 that the lane's row does not see -> `none`.  Behind the sinks a seen key is one range: one subtraction and one
@@ -263,10 +287,18 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
     v16f s[S::KS];
 #pragma unroll
     for (int u = 0; u < S::KS; u++) {
+      Frag8<T> kf[C::KK];
+#pragma unroll
+      for (int kk = 0; kk < C::KK; kk++) kf[kk] = frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h);
+      READS_FIRST;
       s[u] = zero16();
 #pragma unroll
-      for (int kk = 0; kk < C::KK; kk++) s[u] = mma32(frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), qf[kk], s[u]);
+      for (int kk = 0; kk < C::KK; kk++) s[u] = mma32(kf[kk], qf[kk], s[u]);
     }
+    Frag8<T> vf[C::DT];      // the values of the first 16 keys are on their way while the softmax is worked out
+#pragma unroll
+    for (int dt = 0; dt < C::DT; dt++) vf[dt] = tr_frag<T, D>(vs, 0, 32 * dt, lane);
+    READS_FIRST;
     if (!all) {
 #pragma unroll
       for (int u = 0; u < S::KS; u++) mask_keys(s[u], row, k0 + 32 * u, h, a.sinks, -INFINITY);
@@ -293,8 +325,15 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
 #pragma unroll
         for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * st + i], a.c, -mc)); l += p[i]; }
         const Frag8<T> pf = pack8(p, T{});
+        constexpr int last = 2 * S::KS - 1;
+        Frag8<T> vn[C::DT];
+        if (2 * u + st < last) {
 #pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(tr_frag<T, D>(vs, 32 * u + 16 * st, 32 * dt, lane), pf, acc[dt]);
+          for (int dt = 0; dt < C::DT; dt++) vn[dt] = tr_frag<T, D>(vs, 32 * u + 16 * st + 16, 32 * dt, lane);
+          READS_FIRST;
+        }
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) { acc[dt] = mma32(vf[dt], pf, acc[dt]); vf[dt] = vn[dt]; }
       }
   };
 
@@ -308,6 +347,7 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
       sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
     }
     lds_barrier();
+    PROLOGUE_LOADED;
     for (; t < t1; t++) {
       const bool more = t + 1 < t1;
       if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
@@ -337,11 +377,14 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
   T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
   T* vs = ks + S::KT * C::LDP;
   int t = split * per + wv;
-  if (t < t1) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
+  if (S::AHEAD && t < t1) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
   for (; t < t1; t += 4) {
-    sk.store(ks, lane); sv.store(vs, lane);
+    if (!S::AHEAD) sk.load(Kb, a.k.t, key_of(t), sq.len, lane);
+    sk.store(ks, lane);
+    if (!S::AHEAD) sv.load(Vb, a.v.t, key_of(t), sq.len, lane);
+    sv.store(vs, lane);
     wave_lds_sync();
-    if (t + 4 < t1) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
+    if (S::AHEAD && t + 4 < t1) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
     compute(ks, vs, key_of(t));
     wave_lds_sync();
   }
@@ -393,29 +436,31 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
   }
 }
 
-// few rows, many keys: the shares of the key tiles of one row, merged in share order
+// few rows, many keys: the shares of the key tiles of one row, merged in share order.  A wave takes every fourth share; statistics of all
+// shares (at most 64) sit in one register per lane.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void k_win_merge(const WinArgs a) {
-  const int bh = blockIdx.y, r = blockIdx.x, lane = threadIdx.x, b = bh / a.kv, kvh = bh % a.kv;
+__global__ __launch_bounds__(256) void k_win_merge(const WinArgs a) {
+  __shared__ float part[4][D];
+  const int bh = blockIdx.y, r = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, b = bh / a.kv, kvh = bh % a.kv;
   const float* ws = a.part + ((int64_t)bh * a.nsplit * a.rows + r) * (D + 4);
   const int64_t step = (int64_t)a.rows * (D + 4);
-  float M = -INFINITY;
-  for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, ws[s * step + D]);
-  const float Ms = M == -INFINITY ? 0.f : M;
-  float L = 0.f, v[2] = {0.f, 0.f};
-  for (int s = 0; s < a.nsplit; s++) {
-    const float* p = ws + s * step;
-    const float e = __builtin_amdgcn_exp2f(p[D] - Ms);
-    L += p[D + 1] * e;
+  const float m = lane < a.nsplit ? ws[lane * step + D] : -INFINITY, l = lane < a.nsplit ? ws[lane * step + D + 1] : 0.f;
+  const float M = wave_max(m), Ms = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m - Ms), L = wave_sum(l * e);
+  float v[2] = {0.f, 0.f};
+#pragma unroll 4
+  for (int s = wv; s < a.nsplit; s += 4) {
+    const float f = __shfl(e, s, 64);
 #pragma unroll
-    for (int k = 0; k < 2; k++) if (lane + 64 * k < D) v[k] += p[lane + 64 * k] * e;
+    for (int k = 0; k < (D + 63) / 64; k++) if (lane + 64 * k < D) v[k] += ws[s * step + lane + 64 * k] * f;
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int i = r / a.group, g = r - i * a.group;
-  T* o = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)i * a.o.t + (int64_t)(kvh * a.group + g) * a.o.h;
 #pragma unroll
-  for (int k = 0; k < 2; k++) if (lane + 64 * k < D) st_f(o + lane + 64 * k, v[k] * inv);
-  if (lane == 0 && a.lse) a.lse[(int64_t)bh * a.rows + r] = L != 0.f ? Ms + __builtin_amdgcn_logf(L) : INFINITY;
+  for (int k = 0; k < (D + 63) / 64; k++) if (lane + 64 * k < D) part[wv][lane + 64 * k] = v[k];
+  __syncthreads();
+  const int i = r / a.group, g = r - i * a.group;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* o = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)i * a.o.t + (int64_t)(kvh * a.group + g) * a.o.h;
+  if (threadIdx.x < D) st_f(o + threadIdx.x, (part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]) * inv);
+  if (threadIdx.x == 0 && a.lse) a.lse[(int64_t)bh * a.rows + r] = L != 0.f ? Ms + __builtin_amdgcn_logf(L) : INFINITY;
 }
 
 template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t off, int f32, const float* v) {
@@ -468,11 +513,11 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
 #pragma unroll
     for (int u = 0; u < S::KS; u++) {
       v16f s = zero16(), dp = zero16();
+      two_products<T, D>(ks + (32 * u + c32) * C::LDP + 8 * h, vs + (32 * u + c32) * C::LDP + 8 * h, qf, gf, s, dp);
+      Frag8<T> kt[2][C::DT];
 #pragma unroll
-      for (int kk = 0; kk < C::KK; kk++) {
-        s = mma32(frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), qf[kk], s);
-        dp = mma32(frag_ld_lds(vs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), gf[kk], dp);
-      }
+      for (int dt = 0; dt < C::DT; dt++) kt[0][dt] = tr_frag<T, D>(ks, 32 * u, 32 * dt, lane);
+      READS_FIRST;
 #pragma unroll
       for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, ds0);
       if (!all) mask_keys(s, row, k0 + 32 * u, h, a.sinks, 0.f);
@@ -482,8 +527,13 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
 #pragma unroll
         for (int i = 0; i < 8; i++) p[i] = s[8 * st + i];
         const Frag8<T> pf = pack8(p, T{});
+        if (st == 0) {
 #pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(tr_frag<T, D>(ks, 32 * u + 16 * st, 32 * dt, lane), pf, acc[dt]);
+          for (int dt = 0; dt < C::DT; dt++) kt[1][dt] = tr_frag<T, D>(ks, 32 * u + 16, 32 * dt, lane);
+          READS_FIRST;
+        }
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(kt[st][dt], pf, acc[dt]);
       }
     }
   };
@@ -499,6 +549,7 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
       sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
     }
     lds_barrier();
+    PROLOGUE_LOADED;
     for (; t < pl.nt; t++) {
       const bool more = t + 1 < pl.nt;
       if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
@@ -523,11 +574,14 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
   T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
   T* vs = ks + S::KT * C::LDP;
   int t = wv;
-  if (t < pl.nt) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
+  if (S::AHEAD && t < pl.nt) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
   for (; t < pl.nt; t += 4) {
-    sk.store(ks, lane); sv.store(vs, lane);
+    if (!S::AHEAD) sk.load(Kb, a.k.t, key_of(t), sq.len, lane);
+    sk.store(ks, lane);
+    if (!S::AHEAD) sv.load(Vb, a.v.t, key_of(t), sq.len, lane);
+    sv.store(vs, lane);
     wave_lds_sync();
-    if (t + 4 < pl.nt) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
+    if (S::AHEAD && t + 4 < pl.nt) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
     compute(ks, vs, key_of(t));
     wave_lds_sync();
   }
@@ -617,34 +671,44 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
       if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
       const bool all = r0 >= all_lo && r0 + 32 <= all_hi;
       v16f s = zero16(), dp = zero16();
+      two_products<T, D>(qs + (32 * u + c32) * C::LDP + 8 * h, gs + (32 * u + c32) * C::LDP + 8 * h, kf, vf, s, dp);
+      v4f ls[4], dl[4];
 #pragma unroll
-      for (int kk = 0; kk < C::KK; kk++) {
-        s = mma32(frag_ld_lds(qs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), kf[kk], s);
-        dp = mma32(frag_ld_lds(gs + (32 * u + c32) * C::LDP + 16 * kk + 8 * h), vf[kk], dp);
-      }
+      for (int q = 0; q < 4; q++) { ls[q] = *(const v4f*)(sl + 32 * u + 8 * q + 4 * h); dl[q] = *(const v4f*)(sd + 32 * u + 8 * q + 4 * h); }
+      Frag8<T> gt[C::DT], qt[C::DT];
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        const v4f ls = *(const v4f*)(sl + 32 * u + 8 * q + 4 * h), dl = *(const v4f*)(sd + 32 * u + 8 * q + 4 * h);
+      for (int dt = 0; dt < C::DT; dt++) { gt[dt] = tr_frag<T, D>(gs, 32 * u, 32 * dt, lane); qt[dt] = tr_frag<T, D>(qs, 32 * u, 32 * dt, lane); }
+      READS_FIRST;
+      if (!all) {
+        const int off = r0 + 4 * h - mine.lo;
+        const unsigned span = (unsigned)(mine.hi - mine.lo);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[4 * q + i], a.c, -ls[i])), d = p * fmaf(dp[4 * q + i], a.scale, -dl[i]);
-          if (!all) {
-            const bool see = (unsigned)(r0 + 8 * q + 4 * h + i - mine.lo) < (unsigned)(mine.hi - mine.lo);
-            p = see ? p : 0.f; d = see ? d : 0.f;
-          }
-          s[4 * q + i] = p; dp[4 * q + i] = d;
+        for (int i = 0; i < 16; i++) {
+          const bool see = (unsigned)(off + 8 * (i >> 2) + (i & 3)) < span;
+          s[i] = see ? s[i] : -INFINITY; dp[i] = see ? dp[i] : 0.f;
         }
       }
 #pragma unroll
       for (int st = 0; st < 2; st++) {
         float p[8], d[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) { p[i] = s[8 * st + i]; d[i] = dp[8 * st + i]; }
+        for (int i = 0; i < 8; i++) {
+          const int q = 2 * st + (i >> 2);
+          p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -ls[q][i & 3]));
+          d[i] = p[i] * fmaf(dp[8 * st + i], a.scale, -dl[q][i & 3]);
+        }
         const Frag8<T> pf = pack8(p, T{}), df = pack8(d, T{});
+        Frag8<T> gn[C::DT], qn[C::DT];
+        if (st == 0) {
+#pragma unroll
+          for (int dt = 0; dt < C::DT; dt++) { gn[dt] = tr_frag<T, D>(gs, 32 * u + 16, 32 * dt, lane); qn[dt] = tr_frag<T, D>(qs, 32 * u + 16, 32 * dt, lane); }
+          READS_FIRST;
+        }
 #pragma unroll
         for (int dt = 0; dt < C::DT; dt++) {
-          av[dt] = mma32(tr_frag<T, D>(gs, 32 * u + 16 * st, 32 * dt, lane), pf, av[dt]);
-          ak[dt] = mma32(tr_frag<T, D>(qs, 32 * u + 16 * st, 32 * dt, lane), df, ak[dt]);
+          av[dt] = mma32(gt[dt], pf, av[dt]);
+          ak[dt] = mma32(qt[dt], df, ak[dt]);
+          if (st == 0) { gt[dt] = gn[dt]; qt[dt] = qn[dt]; }
         }
       }
     }
@@ -676,6 +740,7 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
     int t = chunk * per, buf = 0;
     if (t < t1) { load(base_r + t * S::RT); store(qs_of(0), qs_of(0) + S::RT * C::LDP, sl_of(0), sl_of(0) + S::RT); }
     lds_barrier();
+    PROLOGUE_LOADED;
     for (; t < t1; t++) {
       const bool more = t + 1 < t1;
       if (more) load(base_r + (t + 1) * S::RT);
@@ -700,11 +765,12 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
     return;
   }
   int t = chunk * per + wv;
-  if (t < t1) load(base_r + t * S::RT);
+  if (S::AHEAD && t < t1) load(base_r + t * S::RT);
   for (; t < t1; t += 4) {
+    if (!S::AHEAD) load(base_r + t * S::RT);
     store(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT);
     wave_lds_sync();
-    if (t + 4 < t1) load(base_r + (t + 4) * S::RT);
+    if (S::AHEAD && t + 4 < t1) load(base_r + (t + 4) * S::RT);
     compute(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT, base_r + t * S::RT);
     wave_lds_sync();
   }
@@ -818,7 +884,7 @@ template <typename T, int D, bool WIDE> int run_fwd(const WinArgs& a, int B, hip
   hipLaunchKernelGGL(kern, dim3(a.tiles * a.nsplit * B * a.kv), dim3(256), smem, st, a);
   DP_CHECK_LAUNCH("window_attention_fwd");
   if (a.nsplit > 1) {
-    hipLaunchKernelGGL((k_win_merge<T, D>), dim3(a.rows, B * a.kv), dim3(64), 0, st, a);
+    hipLaunchKernelGGL((k_win_merge<T, D>), dim3(a.rows, B * a.kv), dim3(256), 0, st, a);
     DP_CHECK_LAUNCH("window_attention_fwd(merge)");
   }
   return 0;
