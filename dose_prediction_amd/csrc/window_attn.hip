@@ -33,6 +33,15 @@ __device__ __forceinline__ v16f mma32(const Frag8<float>& a, const Frag8<float>&
   for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
   return c;
 }
+// Results of matrix instructions, ready to be read by others.  The wait states are written out (18 behind a 16-pass fp32 instruction, 12 behind an
+// 8-pass 16-bit one) and tied to the registers: where a branch stands between the matrix instruction and the first read, the compiler has counted
+// them along the longer of two paths and read the last rows of a tile too early.
+template <typename T> __device__ __forceinline__ void mma_ready(v16f& x) {
+  if constexpr (sizeof(T) == 4) asm volatile("s_nop 15\n\ts_nop 1" : "+v"(x)); else asm volatile("s_nop 11" : "+v"(x));
+}
+template <typename T> __device__ __forceinline__ void mma_ready(v16f& x, v16f& y) {
+  if constexpr (sizeof(T) == 4) asm volatile("s_nop 15\n\ts_nop 1" : "+v"(x), "+v"(y)); else asm volatile("s_nop 11" : "+v"(x), "+v"(y));
+}
 __device__ __forceinline__ v16f zero16() { v16f z; for (int i = 0; i < 16; i++) z[i] = 0.f; return z; }
 
 template <typename T> __device__ __forceinline__ Frag8<T> ldg8(const T* p) { Frag8<T> f; f.u = *(const v4u*)p; return f; }
@@ -74,38 +83,116 @@ __device__ __forceinline__ float pair_sum(float v) {
 }
 
 template <typename T, int D> struct Cfg {
-  static constexpr int ES = sizeof(T);
-  // LDS row pitch (elements): 16-byte reads of 8 consecutive rows and the 4-row x 32-byte blocks of a transposing read fall into
-  // different banks
-  static constexpr int LDP = ES == 4 ? D + 4 : D == 32 ? 56 : D == 64 ? 72 : D == 96 ? 104 : 144;
-  static constexpr int PPR = D * ES / 16, EPP = 16 / ES;       // 16-byte pieces of a row, elements of a piece
+  static constexpr int ES = sizeof(T), PITCH = D * ES;         // bytes of a row in LDS: no padding, the copies below write 1 KB runs
+  static constexpr int PPR = PITCH / 16, SW = PPR % 8 == 0 ? 7 : 3;
   static constexpr int KK = D / 16, DT = D / 32, CP = D + 4;   // k steps, output tiles, fp32 pitch of the merge tile
 };
 
-// k-major operand of the second product: 16 streamed rows from row0 on (k slots in the order of the accumulator registers: 4 h .. 4 h + 3,
-// 8 + 4 h .. 8 + 4 h + 3 of lane half h), channels col0 + (lane & 31)
-template <typename T, int D> __device__ __forceinline__ Frag8<T> tr_frag(const T* tile, int row0, int col0, int lane) {
-  const int r = lane & 15, h = lane >> 5;
-  return tr_pair<8 * Cfg<T, D>::LDP, T>(tile + (row0 + 4 * h + (r >> 2)) * Cfg<T, D>::LDP + col0 + 16 * ((lane >> 4) & 1) + 4 * (r & 3));
+// Tiles go from memory to LDS without passing registers (buffer_load ... lds: 64 lanes x 16 bytes to consecutive LDS addresses).  What keeps
+// the reads free of bank conflicts is the order of a row's 16-byte pieces: piece c of row r stands in place c ^ (r & SW), chosen by the
+// address each lane loads from.  Rows behind `left` are out of the descriptor's range and arrive as zeros.
+typedef int v4i __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4i rsrc_of(const void* p, unsigned bytes) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  return (v4i){__builtin_amdgcn_readfirstlane((int)u), __builtin_amdgcn_readfirstlane((int)(u >> 32)), __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
 }
-#define TR_F32(D) template <> __device__ __forceinline__ Frag8<float> tr_frag<float, D>(const float* tile, int row0, int col0, int lane) { \
-    constexpr int P = Cfg<float, D>::LDP; \
-    const float* p = tile + (row0 + 4 * (lane >> 5)) * P + col0 + (lane & 31); \
-    Frag8<float> f; \
-    f.v[0] = p[0]; f.v[1] = p[P]; f.v[2] = p[2 * P]; f.v[3] = p[3 * P]; f.v[4] = p[8 * P]; f.v[5] = p[9 * P]; f.v[6] = p[10 * P]; f.v[7] = p[11 * P]; \
-    return f; }
-TR_F32(32) TR_F32(64) TR_F32(96) TR_F32(128)
-#undef TR_F32
+// In assembly (no register is loaded, so nothing can be reused too early) because the compiler would wait for every copy under way in front of
+// each transposing LDS read, whatever tile it reads; the waits are written out in stream_tiles.  (s_nop: the descriptor may come from vector
+// instructions, whose scalar results a buffer load must not read for five states; M0 needs one.)
+__device__ __forceinline__ void lds_copy(v4i rs, char* lds, int off) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs) : "memory");
+}
+// DIRECT false: through registers, for tiles beyond the 64 KB of LDS that such a copy can address
+template <typename T, int D, int ROWS, int NTH, bool DIRECT> struct Copy {
+  using C = Cfg<T, D>;
+  static constexpr int NP = ROWS * C::PPR / NTH;
+  static_assert(NP * NTH == ROWS * C::PPR, "every piece of a tile has a thread");
+  int off[NP], stride;       // stride: bytes between rows
+  __device__ __forceinline__ Copy(int64_t st, int gid) : stride((int)st * C::ES) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      const int idx = gid + i * NTH, row = idx / C::PPR;
+      off[i] = row * stride + (((idx % C::PPR) ^ (row & C::SW)) << 4);
+    }
+  }
+  // rows first .. first + ROWS - 1 of `base`, of which `left` exist
+  __device__ __forceinline__ void issue(const T* base, int64_t st, int first, int left, char* lds, int wave) const {
+    const auto rs = rsrc_of(base + (int64_t)first * st, (unsigned)(min(left, ROWS) * stride));
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+      if (DIRECT) lds_copy(rs, lds + (i * NTH + wave * 64) * 16, off[i]);
+    if (!DIRECT) {
+      const auto rb = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)first * st), 0, min(left, ROWS) * stride, 0x00020000);
+      v4u r[NP];
+#pragma unroll
+      for (int i = 0; i < NP; i++) r[i] = __builtin_amdgcn_raw_buffer_load_b128(rb, off[i], 0, 0);
+#pragma unroll
+      for (int i = 0; i < NP; i++) *(v4u*)(lds + (i * NTH + (threadIdx.x & (NTH - 1))) * 16) = r[i];
+    }
+  }
+};
+// this wave's copies have landed
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// this wave's LDS reads are done: their tile may be filled again
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// operand fragments of a staged tile
+template <typename T, int D> struct Frags {
+  using C = Cfg<T, D>;
+  int row, fx, tr, tx;
+  __device__ __forceinline__ Frags(int lane) {
+    const int c32 = lane & 31, h = lane >> 5, r = lane & 15, f = c32 & C::SW;
+    row = c32 * C::PITCH;
+    fx = C::ES == 2 ? h ^ f : (2 * h) ^ f;
+    if (C::ES == 2) {      // four rows of 16 channels per 16 lanes, transposed on the way
+      const int tr_row = 4 * h + (r >> 2);
+      tr = tr_row * C::PITCH + 8 * (r & 1);
+      tx = (2 * ((lane >> 4) & 1) + ((r >> 1) & 1)) ^ (tr_row & C::SW);
+    } else {
+      tr = 4 * h * C::PITCH + 4 * (c32 & 3);
+      tx = (c32 >> 2) ^ (4 * h);
+    }
+  }
+  // row (lane & 31) of the 32 rows from r0 on, channels 16 kk + 8 (lane >> 5) .. + 7
+  __device__ __forceinline__ Frag8<T> rows(const char* tile, int r0, int kk) const {
+    const char* p = tile + r0 * C::PITCH + row;
+    if constexpr (C::ES == 2) { Frag8<T> f; f.u = *(const v4u*)(p + (((2 * kk) ^ fx) << 4)); return f; }
+    else {
+      const v4f a = *(const v4f*)(p + (((4 * kk) ^ fx) << 4)), b = *(const v4f*)(p + (((4 * kk + 1) ^ fx) << 4));
+      Frag8<T> f;
+      f.v[0] = a[0]; f.v[1] = a[1]; f.v[2] = a[2]; f.v[3] = a[3]; f.v[4] = b[0]; f.v[5] = b[1]; f.v[6] = b[2]; f.v[7] = b[3];
+      return f;
+    }
+  }
+  // k-major: channel 32 dt + (lane & 31) of the 16 rows from r0 on, in the order of the accumulator registers (rows 4 h .. 4 h + 3 and
+  // 8 + 4 h .. 8 + 4 h + 3 of lane half h)
+  __device__ __forceinline__ Frag8<T> cols(const char* tile, int r0, int dt) const {
+    const char* p = tile + r0 * C::PITCH + tr;
+    if constexpr (C::ES == 2) return tr_pair<8 * D, T>((const T*)(p + (((4 * dt) ^ tx) << 4)));
+    else {
+      Frag8<T> f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const char* q = p + j * C::PITCH + 128 * dt + ((tx ^ j) << 4);
+        f.v[j] = *(const float*)q; f.v[4 + j] = *(const float*)(q + 8 * C::PITCH);
+      }
+      return f;
+    }
+  }
+};
 
 // Waves per SIMD that the register budget is cut for.  Two (256 registers) also keep the matrix accumulators in plain VGPRs: with more the
 // compiler puts them into AGPRs and copies them back and forth around every rescale and mask (24 instead of 9 vector instructions per
 // matrix instruction in the forward kernel).  One where two would spill.
-template <typename T, int D> constexpr int waves_q() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
+template <typename T, int D> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
+template <typename T, int D> constexpr int waves_dq() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
 template <typename T, int D> constexpr int waves_kv() { return D >= 96 || (sizeof(T) == 4 && D >= 64) ? 1 : 2; }
+
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
   Mat q, k, v, o, go, dq, dk, dv;
-  float *lse, *delta, *part;
+  float *lse, *delta, *part;      // delta: rowsum(dO O) * scale
   const int *starts, *lens;
   int kv, group, Nq, Nk, rows, left, right, sinks, start, tiles, nsplit, sink_tiles, nchunk, g_f32;
   float c, scale;
@@ -125,64 +212,21 @@ __device__ __forceinline__ Seq sequence(const WinArgs& a, int b) {
   return s;
 }
 
-// 32 * KS keys of a matrix, zeros behind `len`: global -> registers -> LDS, by NTH threads
-template <typename T, int D, int KT, int NTH> struct Stage {
-  using C = Cfg<T, D>;
-  static constexpr int NP = KT * C::PPR / NTH;
-  static_assert(NP * NTH == KT * C::PPR, "every piece of a tile has a thread");
-  v4u r[NP];
-  __device__ __forceinline__ void load(const T* base, int64_t st, int k0, int len, int gid) {
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int idx = gid + i * NTH, row = idx / C::PPR, c = idx % C::PPR, key = k0 + row;
-      r[i] = (v4u){0, 0, 0, 0};
-      if (key < len) r[i] = *(const v4u*)(base + (int64_t)key * st + c * C::EPP);
-    }
-  }
-  __device__ __forceinline__ void load_rows(const T* base, int64_t st, int64_t sh, int group, int r0, int rlo, int rhi, int gid) {
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int idx = gid + i * NTH, row = r0 + idx / C::PPR, c = idx % C::PPR;
-      r[i] = (v4u){0, 0, 0, 0};
-      if (row >= rlo && row < rhi) {
-        const int t = group == 1 ? row : row / group;
-        r[i] = *(const v4u*)(base + (int64_t)t * st + (int64_t)(row - t * group) * sh + c * C::EPP);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(T* dst, int gid) const {
-#pragma unroll
-    for (int i = 0; i < NP; i++) {
-      const int idx = gid + i * NTH, row = idx / C::PPR, c = idx % C::PPR;
-      *(v4u*)(dst + row * C::LDP + c * C::EPP) = r[i];
-    }
-  }
-};
-
-// a wave's own LDS writes before its own reads (no other wave is concerned)
-__device__ __forceinline__ void wave_lds_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
-
 template <typename T, int D, bool WIDE> struct Shape {
   using C = Cfg<T, D>;
-  // WIDE: four waves own 32 rows each and share every staged tile (two LDS buffers, one barrier per tile).  Otherwise all four own the same
-  // 32 rows, stream different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
-  static constexpr int KS = (WIDE && C::ES == 2) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64, NBUF = WIDE ? 2 : 1;
-  // the next tile waits in registers while this one is worked on: not in the narrow fp32 kernels, where it would spill (a wave has few tiles)
-  static constexpr bool AHEAD = WIDE || C::ES == 2;
-  static constexpr size_t tile = (size_t)KT * C::LDP * C::ES;
-  static constexpr size_t stage = WIDE ? 2 * NBUF * tile : 4 * 2 * tile;
-  static constexpr size_t merge = WIDE ? 0 : (size_t)4 * 32 * C::CP * 4;
-  static constexpr size_t big = stage > merge ? stage : merge;
-  static constexpr size_t fwd = big + (WIDE ? 0 : 2 * 4 * 32 * 4);
-  // dK / dV: tiles of query rows
-  static constexpr int QS = (WIDE && C::ES == 2 && D <= 96) ? 2 : 1, RT = 32 * QS;
-  static constexpr size_t rtile = (size_t)RT * C::LDP * C::ES;
-  static constexpr size_t rstage = (WIDE ? NBUF : 4) * (2 * rtile + 2 * RT * 4);
-  static constexpr size_t kvb = rstage > merge ? rstage : merge;
+  // WIDE: four waves own 32 rows each and share every staged tile (one barrier per tile).  Otherwise all four own the same 32 rows, stream
+  // different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
+  static constexpr int KS = (WIDE && C::ES == 2) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64;
+  // tiles in LDS per stream: the next one arrives while one is worked on (narrow: where two still leave room for two blocks on a CU)
+  static constexpr int NBUF = WIDE || (C::ES == 2 && D <= 64) ? 2 : 1;
+  static constexpr int tile = KT * C::PITCH, sets = (WIDE ? 1 : 4) * NBUF, stage = sets * 2 * tile;
+  static constexpr bool DIRECT = stage <= 64 * 1024;
+  static constexpr int merge = WIDE ? 0 : 4 * 32 * C::CP * 4, big = stage > merge ? stage : merge;
+  static constexpr int fwd = big + (WIDE ? 0 : 2 * 4 * 32 * 4);
+  // dK / dV: tiles of RT query rows and of the output's gradient, their lse and delta behind all tiles
+  static constexpr int RS = (WIDE && C::ES == 2 && D < 128) ? 2 : 1, RT = 32 * RS, rtile = RT * C::PITCH, rstage = sets * 2 * rtile;
+  static constexpr int kv_all = rstage + sets * 512, kvb = kv_all > merge ? kv_all : merge;
+  static_assert(fwd <= 160 * 1024 && kvb <= 160 * 1024, "LDS of a CU");
 };
 
 // the tiles of KT keys that rows at positions [p0, p1] see at all: `nsink` from key 0 on, then from tile w0 on, nt in all
@@ -210,23 +254,31 @@ __device__ __forceinline__ Row row_of(const WinArgs& a, const Seq& s, int r) {
   w.lo = w.live ? w.p - a.left : 0;
   return w;
 }
+// ... and what a wave's rows see of 32 keys: nothing, all of it, or some
+struct Rows {
+  int p0, p1; bool any;
+  __device__ __forceinline__ Rows(const WinArgs& a, const Seq& s, int r0) : p0(s.start + r0 / a.group), p1(s.start + min(r0 + 31, a.rows - 1) / a.group), any(r0 < a.rows) {}
+  __device__ __forceinline__ bool none(const WinArgs& a, int k0) const { return !any || k0 > p1 + a.right || (k0 + 31 < p0 - a.left && k0 >= a.sinks); }
+  __device__ __forceinline__ bool all(const WinArgs& a, const Seq& s, int k0) const {
+    return k0 + 31 <= min(p0 + a.right, s.len - 1) && (k0 >= p1 - a.left || k0 + 32 <= a.sinks);
+  }
+};
 
-// The LDS reads written above this line are issued before what follows: left alone, the compiler reads each operand right in front of its
-// matrix instruction and waits out the LDS latency every time.
-// (fp32 operands take twice the registers: there the compiler's own order stays)
+// LDS reads written above this line are issued before what follows: left alone, the compiler reads each operand right in front of its matrix
+// instruction and waits out the LDS latency every time.  (fp32 operands take twice the registers: there the compiler's own order stays.)
 #define READS_FIRST do { if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0); } while (0)
-// Loads of the prologue are waited for here: otherwise the waits for them sit inside the loop, where they hold up the prefetch instead.
+// Loads of the prologue are waited for before the loop: otherwise the waits for them sit inside it and hold up the copies instead.
 #define PROLOGUE_LOADED __builtin_amdgcn_s_waitcnt(0)
 
-// s += X x, t += Y y over the head dimension: rows of two staged tiles (x0, y0: the lane's first piece) against fragments in registers
+// s += X x, t += Y y over the head dimension: 32 rows from r0 on of two staged tiles against fragments in registers
 template <typename T, int D>
-__device__ __forceinline__ void two_products(const T* x0, const T* y0, const Frag8<T>* x, const Frag8<T>* y, v16f& s, v16f& t) {
-  constexpr int KK = Cfg<T, D>::KK, G = sizeof(T) == 4 ? 1 : KK < 4 ? KK : KK == 6 ? 3 : 4;      // (an fp32 operand is twice the registers)
+__device__ __forceinline__ void two_products(const Frags<T, D>& F, const char* x0, const char* y0, int r0, const Frag8<T>* x, const Frag8<T>* y, v16f& s, v16f& t) {
+  constexpr int KK = Cfg<T, D>::KK, G = sizeof(T) == 4 ? 1 : KK < 4 ? KK : KK == 6 ? 3 : 4;
 #pragma unroll
   for (int g = 0; g < KK; g += G) {
     Frag8<T> xf[G], yf[G];
 #pragma unroll
-    for (int i = 0; i < G; i++) { xf[i] = frag_ld_lds(x0 + 16 * (g + i)); yf[i] = frag_ld_lds(y0 + 16 * (g + i)); }
+    for (int i = 0; i < G; i++) { xf[i] = F.rows(x0, r0, g + i); yf[i] = F.rows(y0, r0, g + i); }
     READS_FIRST;
 #pragma unroll
     for (int i = 0; i < G; i++) { s = mma32(xf[i], x[g + i], s); t = mma32(yf[i], y[g + i], t); }
@@ -250,9 +302,43 @@ __device__ __forceinline__ void mask_keys(v16f& s, const Row& row, int k0, int h
   for (int i = 0; i < 16; i++) s[i] = (unsigned)(off + 8 * (i >> 2) + (i & 3)) <= span ? s[i] : none;
 }
 
+// The stream of a block's tiles: tile(t, i) issues the copies of tile t into buffer i, land(i) stores what came in registers, work(t, i)
+// computes.  Two buffers: the copies of the next tile run while this one is worked on.  Wide: a wave passes the barrier when its own copies
+// have landed, so behind it everyone's have, and everyone is done with the buffer that is filled next.  Narrow: a wave by itself, every
+// fourth tile.
+template <typename S, typename TILE, typename LAND, typename WORK>
+__device__ __forceinline__ void stream_tiles(int t0, int t1, TILE tile, LAND land, WORK work) {
+  constexpr int step = S::NTH == 256 ? 1 : 4;
+  if (S::NBUF == 2) {
+    int buf = 0;
+    if (t0 < t1) tile(t0, 0);
+    PROLOGUE_LOADED;
+    for (int t = t0; t < t1; t += step) {
+      loads_done();
+      land(buf);
+      if (S::NTH == 256) lds_barrier(); else reads_done();
+      if (t + step < t1) tile(t + step, buf ^ 1);
+      work(t, buf);
+      buf ^= 1;
+    }
+    return;
+  }
+  for (int t = t0; t < t1; t += step) {
+    reads_done();
+    tile(t, 0);
+    loads_done();
+    land(0);
+    work(t, 0);
+  }
+}
+
+template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t off, int f32, const float* v) {
+  if (f32) st4((float*)p + off, v); else st4((T*)p + off, v);
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_fwd<T, D>())) void k_win_fwd(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -263,6 +349,7 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
   const Seq sq = sequence(a, b);
   const int wr0 = WIDE ? r0 + 32 * wv : r0;
   const Row row = row_of(a, sq, wr0 + c32);
+  const Rows wave(a, sq, wr0);
   const T* Kb = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)kvh * a.k.h;
   const T* Vb = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)kvh * a.v.h;
   const T* Qr = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)row.i * a.q.t + (int64_t)(kvh * a.group + row.g) * a.q.h;
@@ -274,42 +361,35 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
   for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
   float m = -INFINITY, mc = 0.f, l = 0.f;
   const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
-  const int per = (pl.nt + a.nsplit - 1) / a.nsplit, t1 = min(pl.nt, (split + 1) * per);
-  // positions of the wave's first and last row (none: nothing to compute, but its threads stage for the others)
-  const bool rows_here = wr0 < a.rows;
-  const int pw0 = sq.start + wr0 / a.group, pw1 = sq.start + min(wr0 + 31, a.rows - 1) / a.group;
+  const int per = (pl.nt + a.nsplit - 1) / a.nsplit, t0 = split * per, t1 = min(pl.nt, t0 + per);
+  const Frags<T, D> F(lane);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
-  auto compute = [&](const T* ks, const T* vs, int k0) {
-    const bool none = !rows_here || k0 > pw1 + a.right || (k0 + S::KT - 1 < pw0 - a.left && k0 >= a.sinks);
-    if (none) return;
-    const bool all = k0 + S::KT - 1 <= min(pw0 + a.right, sq.len - 1) && (k0 >= pw1 - a.left || k0 + S::KT <= a.sinks);
-    v16f s[S::KS];
+  auto step = [&](const char* ks, const char* vs, int u, int k0) {      // 32 keys, k0 the first of them, rows 32 u .. of the tile
+    if (wave.none(a, k0)) return;
+    v16f s = zero16();
+    {
+      constexpr int G = C::KK == 6 ? 3 : C::KK < 4 ? C::KK : 4;
 #pragma unroll
-    for (int u = 0; u < S::KS; u++) {
-      Frag8<T> kf[C::KK];
+      for (int g = 0; g < C::KK; g += G) {
+        Frag8<T> kf[G];
 #pragma unroll
-      for (int kk = 0; kk < C::KK; kk++) kf[kk] = frag_ld_lds(ks + (32 * u + c32) * C::LDP + 16 * kk + 8 * h);
-      READS_FIRST;
-      s[u] = zero16();
+        for (int i = 0; i < G; i++) kf[i] = F.rows(ks, 32 * u, g + i);
+        READS_FIRST;
 #pragma unroll
-      for (int kk = 0; kk < C::KK; kk++) s[u] = mma32(kf[kk], qf[kk], s[u]);
+        for (int i = 0; i < G; i++) s = mma32(kf[i], qf[g + i], s);
+      }
     }
     Frag8<T> vf[C::DT];      // the values of the first 16 keys are on their way while the softmax is worked out
 #pragma unroll
-    for (int dt = 0; dt < C::DT; dt++) vf[dt] = tr_frag<T, D>(vs, 0, 32 * dt, lane);
+    for (int dt = 0; dt < C::DT; dt++) vf[dt] = F.cols(vs, 32 * u, dt);
     READS_FIRST;
-    if (!all) {
+    mma_ready<T>(s);
+    if (!wave.all(a, sq, k0)) mask_keys(s, row, k0, h, a.sinks, -INFINITY);
+    float mx = s[0];
 #pragma unroll
-      for (int u = 0; u < S::KS; u++) mask_keys(s[u], row, k0 + 32 * u, h, a.sinks, -INFINITY);
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int u = 0; u < S::KS; u++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
-    mx = pair_max(mx);
-    const float mn = fmaxf(m, mx);
+    for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+    const float mn = fmaxf(m, pair_max(mx));
     if (__builtin_amdgcn_ballot_w64(mn > m)) {        // (the maximum of a row moves in its first tiles, hardly ever after them)
       // (alpha from the rounded products: exactly 1 for the rows whose maximum stays, whatever the wave's other rows hold)
       const float nc = mn == -INFINITY ? 0.f : mn * a.c, alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - nc);
@@ -318,45 +398,42 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
       for (int dt = 0; dt < C::DT; dt++) acc[dt] *= alpha;
     }
 #pragma unroll
-    for (int u = 0; u < S::KS; u++)
+    for (int st = 0; st < 2; st++) {
+      float p[8];
 #pragma unroll
-      for (int st = 0; st < 2; st++) {
-        float p[8];
+      for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -mc)); l += p[i]; }
+      const Frag8<T> pf = pack8(p, T{});
+      Frag8<T> vn[C::DT];
+      if (st == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * st + i], a.c, -mc)); l += p[i]; }
-        const Frag8<T> pf = pack8(p, T{});
-        constexpr int last = 2 * S::KS - 1;
-        Frag8<T> vn[C::DT];
-        if (2 * u + st < last) {
-#pragma unroll
-          for (int dt = 0; dt < C::DT; dt++) vn[dt] = tr_frag<T, D>(vs, 32 * u + 16 * st + 16, 32 * dt, lane);
-          READS_FIRST;
-        }
-#pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) { acc[dt] = mma32(vf[dt], pf, acc[dt]); vf[dt] = vn[dt]; }
+        for (int dt = 0; dt < C::DT; dt++) vn[dt] = F.cols(vs, 32 * u + 16, dt);
+        READS_FIRST;
       }
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++) { acc[dt] = mma32(vf[dt], pf, acc[dt]); if (st == 0) vf[dt] = vn[dt]; }
+    }
   };
 
-  Stage<T, D, S::KT, S::NTH> sk, sv;
+  const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
+  const Copy<T, D, S::KT, S::NTH, S::DIRECT> ck(a.k.t, gid), cv(a.v.t, gid);
+  char* const tiles = smem + (WIDE ? 0 : wv * S::NBUF * 2 * S::tile);
+  stream_tiles<S>(WIDE ? t0 : t0 + wv, t1,
+    [&](int t, int i) {
+      const int k0 = key_of(t);
+      char* at = tiles + i * 2 * S::tile;
+      ck.issue(Kb, a.k.t, k0, sq.len - k0, at, wave_id); cv.issue(Vb, a.v.t, k0, sq.len - k0, at + S::tile, wave_id);
+    },
+    [](int) {},
+    [&](int t, int i) {
+      const int k0 = key_of(t);
+      const char* at = tiles + i * 2 * S::tile;
+#pragma unroll
+      for (int u = 0; u < S::KS; u++) step(at, at + S::tile, u, k0 + 32 * u);
+    });
+  l = pair_sum(l);
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) mma_ready<T>(acc[dt]);
   if (WIDE) {
-    int t = split * per, buf = 0;
-    T* base = (T*)smem;
-    auto kbuf = [&](int i) { return base + i * 2 * S::KT * C::LDP; };
-    if (t < t1) {
-      sk.load(Kb, a.k.t, key_of(t), sq.len, tid); sv.load(Vb, a.v.t, key_of(t), sq.len, tid);
-      sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
-    }
-    lds_barrier();
-    PROLOGUE_LOADED;
-    for (; t < t1; t++) {
-      const bool more = t + 1 < t1;
-      if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
-      compute(kbuf(buf), kbuf(buf) + S::KT * C::LDP, key_of(t));
-      if (more) { sk.store(kbuf(buf ^ 1), tid); sv.store(kbuf(buf ^ 1) + S::KT * C::LDP, tid); }
-      lds_barrier();
-      buf ^= 1;
-    }
-    l = pair_sum(l);
     if (row.r < a.rows) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* Or = (T*)a.o.p + (int64_t)b * a.o.b + (int64_t)row.i * a.o.t + (int64_t)(kvh * a.group + row.g) * a.o.h;
@@ -374,21 +451,6 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_fwd(const WinArg
     return;
   }
 
-  T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
-  T* vs = ks + S::KT * C::LDP;
-  int t = split * per + wv;
-  if (S::AHEAD && t < t1) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
-  for (; t < t1; t += 4) {
-    if (!S::AHEAD) sk.load(Kb, a.k.t, key_of(t), sq.len, lane);
-    sk.store(ks, lane);
-    if (!S::AHEAD) sv.load(Vb, a.v.t, key_of(t), sq.len, lane);
-    sv.store(vs, lane);
-    wave_lds_sync();
-    if (S::AHEAD && t + 4 < t1) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
-    compute(ks, vs, key_of(t));
-    wave_lds_sync();
-  }
-  l = pair_sum(l);
   if (!row.live) { l = 0.f; m = -INFINITY; }
   float* part = (float*)smem;
   float* mw = (float*)(smem + S::big);
@@ -447,7 +509,6 @@ __global__ __launch_bounds__(256) void k_win_merge(const WinArgs a) {
   const float m = lane < a.nsplit ? ws[lane * step + D] : -INFINITY, l = lane < a.nsplit ? ws[lane * step + D + 1] : 0.f;
   const float M = wave_max(m), Ms = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m - Ms), L = wave_sum(l * e);
   float v[2] = {0.f, 0.f};
-#pragma unroll 4
   for (int s = wv; s < a.nsplit; s += 4) {
     const float f = __shfl(e, s, 64);
 #pragma unroll
@@ -463,13 +524,9 @@ __global__ __launch_bounds__(256) void k_win_merge(const WinArgs a) {
   if (threadIdx.x == 0 && a.lse) a.lse[(int64_t)bh * a.rows + r] = L != 0.f ? Ms + __builtin_amdgcn_logf(L) : INFINITY;
 }
 
-template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t off, int f32, const float* v) {
-  if (f32) st4((float*)p + off, v); else st4((T*)p + off, v);
-}
-
 // ------------------------------------------------------------------------------------------------ backward: dQ (and delta)
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -479,6 +536,7 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
   const Seq sq = sequence(a, b);
   const int wr0 = WIDE ? r0 + 32 * wv : r0;
   const Row row = row_of(a, sq, wr0 + c32);
+  const Rows wave(a, sq, wr0);
   const int head = kvh * a.group + row.g;
   const T* Kb = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)kvh * a.k.h;
   const T* Vb = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)kvh * a.v.h;
@@ -494,70 +552,64 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
 #pragma unroll
     for (int i = 0; i < 8; i++) dl += elem(of, i) * elem(gf[kk], i);
   }
-  dl = pair_sum(dl);
+  dl = pair_sum(dl) * a.scale;
   const float lse = row.live ? a.lse[(int64_t)bh * a.rows + row.r] : INFINITY;
   if (row.r < a.rows && h == 0 && (WIDE || wv == 0)) a.delta[(int64_t)bh * a.rows + row.r] = row.live ? dl : 0.f;
-  const float ds0 = -dl * a.scale;
   v16f acc[C::DT];
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
   const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
-  const bool rows_here = wr0 < a.rows;
-  const int pw0 = sq.start + wr0 / a.group, pw1 = sq.start + min(wr0 + 31, a.rows - 1) / a.group;
+  const Frags<T, D> F(lane);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
-  auto compute = [&](const T* ks, const T* vs, int k0) {
-    const bool none = !rows_here || k0 > pw1 + a.right || (k0 + S::KT - 1 < pw0 - a.left && k0 >= a.sinks);
-    if (none) return;
-    const bool all = k0 + S::KT - 1 <= min(pw0 + a.right, sq.len - 1) && (k0 >= pw1 - a.left || k0 + S::KT <= a.sinks);
+  auto step = [&](const char* ks, const char* vs, int u, int k0) {
+    if (wave.none(a, k0)) return;
+    v16f s = zero16(), dp = zero16();
+    two_products<T, D>(F, ks, vs, 32 * u, qf, gf, s, dp);
+    Frag8<T> kt[2][C::DT];
 #pragma unroll
-    for (int u = 0; u < S::KS; u++) {
-      v16f s = zero16(), dp = zero16();
-      two_products<T, D>(ks + (32 * u + c32) * C::LDP + 8 * h, vs + (32 * u + c32) * C::LDP + 8 * h, qf, gf, s, dp);
-      Frag8<T> kt[2][C::DT];
+    for (int dt = 0; dt < C::DT; dt++) kt[0][dt] = F.cols(ks, 32 * u, dt);
+    READS_FIRST;
+    mma_ready<T>(s, dp);
 #pragma unroll
-      for (int dt = 0; dt < C::DT; dt++) kt[0][dt] = tr_frag<T, D>(ks, 32 * u, 32 * dt, lane);
-      READS_FIRST;
+    for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, -dl);
+    if (!wave.all(a, sq, k0)) mask_keys(s, row, k0, h, a.sinks, 0.f);
 #pragma unroll
-      for (int i = 0; i < 16; i++) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * fmaf(dp[i], a.scale, ds0);
-      if (!all) mask_keys(s, row, k0 + 32 * u, h, a.sinks, 0.f);
+    for (int st = 0; st < 2; st++) {
+      float p[8];
 #pragma unroll
-      for (int st = 0; st < 2; st++) {
-        float p[8];
+      for (int i = 0; i < 8; i++) p[i] = s[8 * st + i];
+      const Frag8<T> pf = pack8(p, T{});
+      if (st == 0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = s[8 * st + i];
-        const Frag8<T> pf = pack8(p, T{});
-        if (st == 0) {
-#pragma unroll
-          for (int dt = 0; dt < C::DT; dt++) kt[1][dt] = tr_frag<T, D>(ks, 32 * u + 16, 32 * dt, lane);
-          READS_FIRST;
-        }
-#pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(kt[st][dt], pf, acc[dt]);
+        for (int dt = 0; dt < C::DT; dt++) kt[1][dt] = F.cols(ks, 32 * u + 16, dt);
+        READS_FIRST;
       }
+#pragma unroll
+      for (int dt = 0; dt < C::DT; dt++) acc[dt] = mma32(kt[st][dt], pf, acc[dt]);
     }
   };
 
-  Stage<T, D, S::KT, S::NTH> sk, sv;
-  const int64_t qoff = (int64_t)b * a.dq.b + (int64_t)row.i * a.dq.t + (int64_t)head * a.dq.h;
+  const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
+  const Copy<T, D, S::KT, S::NTH, S::DIRECT> ck(a.k.t, gid), cv(a.v.t, gid);
+  char* const tiles = smem + (WIDE ? 0 : wv * S::NBUF * 2 * S::tile);
+  stream_tiles<S>(WIDE ? 0 : wv, pl.nt,
+    [&](int t, int i) {
+      const int k0 = key_of(t);
+      char* at = tiles + i * 2 * S::tile;
+      ck.issue(Kb, a.k.t, k0, sq.len - k0, at, wave_id); cv.issue(Vb, a.v.t, k0, sq.len - k0, at + S::tile, wave_id);
+    },
+    [](int) {},
+    [&](int t, int i) {
+      const int k0 = key_of(t);
+      const char* at = tiles + i * 2 * S::tile;
+#pragma unroll
+      for (int u = 0; u < S::KS; u++) step(at, at + S::tile, u, k0 + 32 * u);
+    });
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) mma_ready<T>(acc[dt]);
   if (WIDE) {
-    int t = 0, buf = 0;
-    T* base = (T*)smem;
-    auto kbuf = [&](int i) { return base + i * 2 * S::KT * C::LDP; };
-    if (t < pl.nt) {
-      sk.load(Kb, a.k.t, key_of(t), sq.len, tid); sv.load(Vb, a.v.t, key_of(t), sq.len, tid);
-      sk.store(kbuf(0), tid); sv.store(kbuf(0) + S::KT * C::LDP, tid);
-    }
-    lds_barrier();
-    PROLOGUE_LOADED;
-    for (; t < pl.nt; t++) {
-      const bool more = t + 1 < pl.nt;
-      if (more) { sk.load(Kb, a.k.t, key_of(t + 1), sq.len, tid); sv.load(Vb, a.v.t, key_of(t + 1), sq.len, tid); }
-      compute(kbuf(buf), kbuf(buf) + S::KT * C::LDP, key_of(t));
-      if (more) { sk.store(kbuf(buf ^ 1), tid); sv.store(kbuf(buf ^ 1) + S::KT * C::LDP, tid); }
-      lds_barrier();
-      buf ^= 1;
-    }
+    const int64_t qoff = (int64_t)b * a.dq.b + (int64_t)row.i * a.dq.t + (int64_t)head * a.dq.h;
     if (row.r < a.rows) {
 #pragma unroll
       for (int dt = 0; dt < C::DT; dt++)
@@ -570,20 +622,6 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
         }
     }
     return;
-  }
-  T* ks = (T*)smem + wv * 2 * S::KT * C::LDP;
-  T* vs = ks + S::KT * C::LDP;
-  int t = wv;
-  if (S::AHEAD && t < pl.nt) { sk.load(Kb, a.k.t, key_of(t), sq.len, lane); sv.load(Vb, a.v.t, key_of(t), sq.len, lane); }
-  for (; t < pl.nt; t += 4) {
-    if (!S::AHEAD) sk.load(Kb, a.k.t, key_of(t), sq.len, lane);
-    sk.store(ks, lane);
-    if (!S::AHEAD) sv.load(Vb, a.v.t, key_of(t), sq.len, lane);
-    sv.store(vs, lane);
-    wave_lds_sync();
-    if (S::AHEAD && t + 4 < pl.nt) { sk.load(Kb, a.k.t, key_of(t + 4), sq.len, lane); sv.load(Vb, a.v.t, key_of(t + 4), sq.len, lane); }
-    compute(ks, vs, key_of(t));
-    wave_lds_sync();
   }
   float* part = (float*)smem;
   __syncthreads();
@@ -613,12 +651,12 @@ __global__ __launch_bounds__(256, (waves_q<T, D>())) void k_win_dq(const WinArgs
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
-// query rows [lo, hi) that see key j at all
+// tokens [lo, hi) whose queries see any key of [jlo, jhi], jhi < len
 struct Span { int lo, hi; };
-__device__ __forceinline__ Span rows_of(const WinArgs& a, const Seq& s, int jlo, int jhi) {      // ... that see any key of [jlo, jhi], jhi < len
+__device__ __forceinline__ Span tokens_of(const WinArgs& a, const Seq& s, int jlo, int jhi) {
   const int p0 = max(jlo - a.right, 0), p1 = jlo < a.sinks ? s.len - 1 : min(jhi + a.left, s.len - 1);
   const int i0 = min(max(p0 - s.start, 0), a.Nq), i1 = min(p1 - s.start, a.Nq - 1);
-  return Span{i0 * a.group, i1 < i0 ? i0 * a.group : (i1 + 1) * a.group};
+  return Span{i0, max(i1 + 1, i0)};
 }
 
 template <typename T, int D, bool WIDE>
@@ -650,9 +688,9 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   v16f ak[C::DT], av[C::DT];
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++) { ak[dt] = zero16(); av[dt] = zero16(); }
-  const Span mine = live ? rows_of(a, sq, j, j) : Span{0x7fffffff, 0x7fffffff};
-  const Span block = k0 < sq.len ? rows_of(a, sq, k0, min(k0 + S::ROWS, sq.len) - 1) : Span{0, 0};
-  // (rows that all keys of the wave see need no mask, rows that none of them sees no work)
+  const Span mine = live ? tokens_of(a, sq, j, j) : Span{0x7fffffff, 0x7fffffff};
+  const Span block = k0 < sq.len ? tokens_of(a, sq, k0, min(k0 + S::ROWS, sq.len) - 1) : Span{0, 0};
+  // (tokens that all keys of the wave are seen by need no mask, tokens that see none of them no work)
   int all_lo = mine.lo, all_hi = live ? mine.hi : 0, any_lo = mine.lo, any_hi = live ? mine.hi : 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -661,94 +699,86 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   }
   all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   any_lo = __builtin_amdgcn_readfirstlane(any_lo); any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-  const int base_r = block.lo / S::RT * S::RT, ntile = block.hi > block.lo ? (block.hi - base_r + S::RT - 1) / S::RT : 0;
-  const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t1 = min(ntile, (chunk + 1) * per);
+  // tiles of RT tokens of one query head, the heads of the group one after the other
+  const int per_head = (block.hi - block.lo + S::RT - 1) / S::RT, ntile = per_head * a.group;
+  const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t0 = chunk * per, t1 = min(ntile, t0 + per);
+  const Frags<T, D> F(lane);
 
-  auto compute = [&](const T* qs, const T* gs, const float* sl, const float* sd, int rt) {
+  auto step = [&](const char* qs, const char* gs, const float* sl, const float* sd, int u, int i0) {      // 32 query rows, i0 the first token
+    if (i0 >= any_hi || i0 + 32 <= any_lo) return;
+    v16f s = zero16(), dp = zero16();
+    two_products<T, D>(F, qs, gs, 32 * u, kf, vf, s, dp);
+    Frag8<T> gt[C::DT], qt[C::DT];
 #pragma unroll
-    for (int u = 0; u < S::QS; u++) {
-      const int r0 = rt + 32 * u;
-      if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
-      const bool all = r0 >= all_lo && r0 + 32 <= all_hi;
-      v16f s = zero16(), dp = zero16();
-      two_products<T, D>(qs + (32 * u + c32) * C::LDP + 8 * h, gs + (32 * u + c32) * C::LDP + 8 * h, kf, vf, s, dp);
-      v4f ls[4], dl[4];
+    for (int dt = 0; dt < C::DT; dt++) { gt[dt] = F.cols(gs, 32 * u, dt); qt[dt] = F.cols(qs, 32 * u, dt); }
+    READS_FIRST;
+    mma_ready<T>(s, dp);
+    if (!(i0 >= all_lo && i0 + 32 <= all_hi)) {
+      const int off = i0 + 4 * h - mine.lo;
+      const unsigned span = (unsigned)(mine.hi - mine.lo);
 #pragma unroll
-      for (int q = 0; q < 4; q++) { ls[q] = *(const v4f*)(sl + 32 * u + 8 * q + 4 * h); dl[q] = *(const v4f*)(sd + 32 * u + 8 * q + 4 * h); }
-      Frag8<T> gt[C::DT], qt[C::DT];
+      for (int i = 0; i < 16; i++) {
+        const bool see = (unsigned)(off + 8 * (i >> 2) + (i & 3)) < span;
+        s[i] = see ? s[i] : -INFINITY; dp[i] = see ? dp[i] : 0.f;
+      }
+    }
 #pragma unroll
-      for (int dt = 0; dt < C::DT; dt++) { gt[dt] = tr_frag<T, D>(gs, 32 * u, 32 * dt, lane); qt[dt] = tr_frag<T, D>(qs, 32 * u, 32 * dt, lane); }
+    for (int st = 0; st < 2; st++) {
+      v4f ls[2], dl[2];
+#pragma unroll
+      for (int q = 0; q < 2; q++) { ls[q] = *(const v4f*)(sl + 32 * u + 16 * st + 8 * q + 4 * h); dl[q] = *(const v4f*)(sd + 32 * u + 16 * st + 8 * q + 4 * h); }
       READS_FIRST;
-      if (!all) {
-        const int off = r0 + 4 * h - mine.lo;
-        const unsigned span = (unsigned)(mine.hi - mine.lo);
+      float p[8], d[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const bool see = (unsigned)(off + 8 * (i >> 2) + (i & 3)) < span;
-          s[i] = see ? s[i] : -INFINITY; dp[i] = see ? dp[i] : 0.f;
-        }
+      for (int i = 0; i < 8; i++) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -ls[i >> 2][i & 3]));
+        d[i] = p[i] * fmaf(dp[8 * st + i], a.scale, -dl[i >> 2][i & 3]);
+      }
+      const Frag8<T> pf = pack8(p, T{}), df = pack8(d, T{});
+      Frag8<T> gn[C::DT], qn[C::DT];
+      if (st == 0) {
+#pragma unroll
+        for (int dt = 0; dt < C::DT; dt++) { gn[dt] = F.cols(gs, 32 * u + 16, dt); qn[dt] = F.cols(qs, 32 * u + 16, dt); }
+        READS_FIRST;
       }
 #pragma unroll
-      for (int st = 0; st < 2; st++) {
-        float p[8], d[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int q = 2 * st + (i >> 2);
-          p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -ls[q][i & 3]));
-          d[i] = p[i] * fmaf(dp[8 * st + i], a.scale, -dl[q][i & 3]);
-        }
-        const Frag8<T> pf = pack8(p, T{}), df = pack8(d, T{});
-        Frag8<T> gn[C::DT], qn[C::DT];
-        if (st == 0) {
-#pragma unroll
-          for (int dt = 0; dt < C::DT; dt++) { gn[dt] = tr_frag<T, D>(gs, 32 * u + 16, 32 * dt, lane); qn[dt] = tr_frag<T, D>(qs, 32 * u + 16, 32 * dt, lane); }
-          READS_FIRST;
-        }
-#pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) {
-          av[dt] = mma32(gt[dt], pf, av[dt]);
-          ak[dt] = mma32(qt[dt], df, ak[dt]);
-          if (st == 0) { gt[dt] = gn[dt]; qt[dt] = qn[dt]; }
-        }
+      for (int dt = 0; dt < C::DT; dt++) {
+        av[dt] = mma32(gt[dt], pf, av[dt]);
+        ak[dt] = mma32(qt[dt], df, ak[dt]);
+        if (st == 0) { gt[dt] = gn[dt]; qt[dt] = qn[dt]; }
       }
     }
   };
 
-  Stage<T, D, S::RT, S::NTH> sqr, sgr;
+  const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
+  const Copy<T, D, S::RT, S::NTH, S::DIRECT> cq(a.q.t, gid), cg(a.go.t, gid);
+  const int set0 = WIDE ? 0 : wv * S::NBUF;
   float ls = 0.f, dl = 0.f;
-  const int gid = WIDE ? tid : lane;
-  // rows outside [lo, hi) of the block are staged as zeros with an infinite lse: they add nothing, whatever they hold
-  auto load = [&](int rt) {
-    sqr.load_rows(Qb, a.q.t, a.q.h, a.group, rt, block.lo, block.hi, gid);
-    sgr.load_rows(Gb, a.go.t, a.go.h, a.group, rt, block.lo, block.hi, gid);
-    if (gid < S::RT) {
-      const int r = rt + gid;
-      const bool ok = r >= block.lo && r < block.hi;
-      ls = ok ? lseb[r] : INFINITY; dl = ok ? dlb[r] * a.scale : 0.f;
-    }
-  };
-  auto store = [&](T* qs, T* gs, float* sl, float* sd) {
-    sqr.store(qs, gid); sgr.store(gs, gid);
-    if (gid < S::RT) { sl[gid] = ls; sd[gid] = dl; }
-  };
-  constexpr size_t set = 2 * S::rtile + 2 * S::RT * 4;
-  auto qs_of = [&](int i) { return (T*)(smem + i * set); };
-  auto sl_of = [&](int i) { return (float*)(smem + i * set + 2 * S::rtile); };
+  auto stats_of = [&](int i) { return (float*)(smem + S::rstage + (set0 + i) * 512); };
+  stream_tiles<S>(WIDE ? t0 : t0 + wv, t1,
+    [&](int t, int i) {
+      // rows behind the block's tokens arrive as zeros, with zeros for lse and delta: P = 1 times a zero row of dO, dS = 0
+      const int g = a.group == 1 ? 0 : t / per_head, i0 = block.lo + (t - g * per_head) * S::RT, left = block.hi - i0;
+      char* at = smem + (set0 + i) * 2 * S::rtile;
+      cq.issue(Qb + (int64_t)g * a.q.h, a.q.t, i0, left, at, wave_id); cg.issue(Gb + (int64_t)g * a.go.h, a.go.t, i0, left, at + S::rtile, wave_id);
+      const bool in = gid < min(left, S::RT);
+      const int64_t r = (int64_t)(i0 + (in ? gid : 0)) * a.group + g;
+      ls = in ? lseb[r] : 0.f; dl = in ? dlb[r] : 0.f;
+    },
+    [&](int i) { if (gid < S::RT) { float* st = stats_of(i); st[gid] = ls; st[64 + gid] = dl; } },
+    [&](int t, int i) {
+      const int i0 = block.lo + (a.group == 1 ? t : t % per_head) * S::RT;
+      const char* at = smem + (set0 + i) * 2 * S::rtile;
+      const float* st = stats_of(i);
+#pragma unroll
+      for (int u = 0; u < S::RS; u++) step(at, at + S::rtile, st, st + 64, u, i0 + 32 * u);
+    });
+
+#pragma unroll
+  for (int dt = 0; dt < C::DT; dt++) mma_ready<T>(ak[dt], av[dt]);
   float* ws = shared_rows ? a.part + (((int64_t)bh * a.sink_tiles + tile) * a.nchunk + chunk) * (2 * S::ROWS * D) : nullptr;
   const int64_t koff = (int64_t)b * a.dk.b + (int64_t)kvh * a.dk.h, voff = (int64_t)b * a.dv.b + (int64_t)kvh * a.dv.h;
   if (WIDE) {
-    int t = chunk * per, buf = 0;
-    if (t < t1) { load(base_r + t * S::RT); store(qs_of(0), qs_of(0) + S::RT * C::LDP, sl_of(0), sl_of(0) + S::RT); }
-    lds_barrier();
-    PROLOGUE_LOADED;
-    for (; t < t1; t++) {
-      const bool more = t + 1 < t1;
-      if (more) load(base_r + (t + 1) * S::RT);
-      compute(qs_of(buf), qs_of(buf) + S::RT * C::LDP, sl_of(buf), sl_of(buf) + S::RT, base_r + t * S::RT);
-      if (more) store(qs_of(buf ^ 1), qs_of(buf ^ 1) + S::RT * C::LDP, sl_of(buf ^ 1), sl_of(buf ^ 1) + S::RT);
-      lds_barrier();
-      buf ^= 1;
-    }
     if (j < a.Nk) {
 #pragma unroll
       for (int dt = 0; dt < C::DT; dt++)
@@ -763,16 +793,6 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
         }
     }
     return;
-  }
-  int t = chunk * per + wv;
-  if (S::AHEAD && t < t1) load(base_r + t * S::RT);
-  for (; t < t1; t += 4) {
-    if (!S::AHEAD) load(base_r + t * S::RT);
-    store(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT);
-    wave_lds_sync();
-    if (S::AHEAD && t + 4 < t1) load(base_r + (t + 4) * S::RT);
-    compute(qs_of(wv), qs_of(wv) + S::RT * C::LDP, sl_of(wv), sl_of(wv) + S::RT, base_r + t * S::RT);
-    wave_lds_sync();
   }
   float* part = (float*)smem;
 #pragma unroll
@@ -871,8 +891,11 @@ int check(const char* name, int B, int heads, int kv, int Nq, int Nk, int d, int
     DP_FAIL("%s: too many rows", name);
   return 0;
 }
-int check_mat(const char* name, const char* what, const Mat& m, int es) {
+// n > 0: a matrix of n tokens that is copied to LDS by 32-bit offsets from its tile's first row
+int check_mat(const char* name, const char* what, Mat& m, int es, int n = 0, int d = 0) {
   if (((uintptr_t)m.p & 15) || (m.b * es) % 16 || (m.t * es) % 16 || (m.h * es) % 16) DP_FAIL("%s: %s: rows must be 16-byte aligned", name, what);
+  if (n > 1 && (m.t < d || m.t * es > (1 << 24))) DP_FAIL("%s: %s: token stride %lld (at least the head dim, at most 16 MB)", name, what, (long long)m.t);
+  if (n == 1) m.t = d;
   return 0;
 }
 
@@ -934,7 +957,7 @@ extern "C" int dp_window_attention_fwd(const void* q, int64_t qb, int64_t qt, in
   WinArgs a{};
   a.q = Mat{(void*)q, qb, qt, qh}; a.k = Mat{(void*)k, kb, kt, kh}; a.v = Mat{(void*)v, vb, vt, vh}; a.o = Mat{o, ob, ot, oh};
   const int es = dtype == DP_F32 ? 4 : 2;
-  if (check_mat("window_attention_fwd", "q", a.q, es) || check_mat("window_attention_fwd", "k", a.k, es) || check_mat("window_attention_fwd", "v", a.v, es) ||
+  if (check_mat("window_attention_fwd", "q", a.q, es, B > 0 ? Nq : 0, d) || check_mat("window_attention_fwd", "k", a.k, es, B > 0 ? Nk : 0, d) || check_mat("window_attention_fwd", "v", a.v, es, B > 0 ? Nk : 0, d) ||
       check_mat("window_attention_fwd", "o", a.o, es)) return 1;
   if (B == 0 || Nq == 0) return 0;
   a.lse = lse; a.part = ws; a.starts = q_starts; a.lens = lengths;
@@ -961,8 +984,8 @@ extern "C" int dp_window_attention_bwd(const void* q, int64_t qb, int64_t qt, in
   a.q = Mat{(void*)q, qb, qt, qh}; a.k = Mat{(void*)k, kb, kt, kh}; a.v = Mat{(void*)v, vb, vt, vh}; a.o = Mat{(void*)o, ob, ot, oh};
   a.go = Mat{(void*)go, gb, gt, gh}; a.dq = Mat{dq, dqb, dqt, dqh}; a.dk = Mat{dk, dkb, dkt, dkh}; a.dv = Mat{dv, dvb, dvt, dvh};
   const int es = dtype == DP_F32 ? 4 : 2, gs = qk_f32 ? 4 : es;
-  if (check_mat(name, "q", a.q, es) || check_mat(name, "k", a.k, es) || check_mat(name, "v", a.v, es) || check_mat(name, "o", a.o, es) ||
-      check_mat(name, "go", a.go, es) || check_mat(name, "dq", a.dq, gs) || check_mat(name, "dk", a.dk, gs) || check_mat(name, "dv", a.dv, es)) return 1;
+  if (check_mat(name, "q", a.q, es, B > 0 ? Nq : 0, d) || check_mat(name, "k", a.k, es, B > 0 ? Nk : 0, d) || check_mat(name, "v", a.v, es, B > 0 ? Nk : 0, d) || check_mat(name, "o", a.o, es) ||
+      check_mat(name, "go", a.go, es, B > 0 ? Nq : 0, d) || check_mat(name, "dq", a.dq, gs) || check_mat(name, "dk", a.dk, gs) || check_mat(name, "dv", a.dv, es)) return 1;
   if (B == 0) return 0;
   if (Nq > 0 && (!lse || !delta)) DP_FAIL("%s: lse / delta missing", name);
   a.lse = (float*)lse; a.delta = delta; a.part = ws; a.starts = q_starts; a.lens = lengths;

@@ -2354,14 +2354,17 @@ class _NoGuard:
 _NO_GUARD = _NoGuard()
 
 
-def _strided(t):
-    """(tensor, strides of all but the last dimension): t itself where its last dimension is dense and every row 16-byte aligned, otherwise a
-    contiguous copy."""
-    st, es = t.stride(), t.element_size()
-    if (st[-1] == 1 or t.shape[-1] <= 1) and t.data_ptr() % 16 == 0 and all(n <= 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], st)):
-        return t, [0 if n <= 1 else s for n, s in zip(t.shape[:-1], st)]
+def _strided(t, tiles=False):
+    """(tensor, strides of all but the last dimension): t itself where its last dimension is dense and every row 16-byte aligned (tiles: and
+    its tokens, dimension 1, do not overlap and lie at most 16 MB apart), otherwise a contiguous copy."""
+    st, es, shape = t.stride(), t.element_size(), t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and shape[-1] * es % 16 == 0:
+        return t, st[:-1]
+    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s * es % 16 == 0 for n, s in zip(shape[:-1], st))
+            and not (tiles and shape[1] > 1 and (st[1] < shape[-1] or st[1] * es > 1 << 24))):
+        return t, [0 if n <= 1 else s for n, s in zip(shape[:-1], st)]
     t = t.contiguous() if not t.is_contiguous() else t.clone()
-    return t, [0 if n <= 1 else s for n, s in zip(t.shape[:-1], t.stride())]
+    return t, t.stride()[:-1]
 
 
 def _head_dim(width, heads, what):
@@ -2531,7 +2534,7 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, win, start, starts, lengths):
-        (qs, qst), (ks, kst), (vs, vst) = _strided(q), _strided(k), _strided(v)
+        (qs, qst), (ks, kst), (vs, vst) = _strided(q, True), _strided(k, True), _strided(v, True)
         (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
         o = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
         need = any(ctx.needs_input_grad[:3])
@@ -2549,7 +2552,7 @@ class WindowAttention(torch.autograd.Function):
     def backward(ctx, g):
         q, k, v, o, lse, starts, lengths = ctx.saved_tensors
         qst, kst, vst, win, start = ctx.opts
-        gs, gst = _strided(g)
+        gs, gst = _strided(g, True)
         (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
         dq = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
         dk = torch.empty((B, Nk, kv, d), dtype=q.dtype, device=q.device)
@@ -2599,7 +2602,7 @@ class WindowAttentionQkv(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, qw, qb, kw, kb, heads, kv, eps, positions, rot, win, lengths):
-        xs, (xb, xt) = _strided(qkv)
+        xs, (xb, xt) = _strided(qkv, True)
         B, N, W = qkv.shape
         d, es, dtc = W // (heads + 2 * kv), qkv.element_size(), _dt(qkv)
         Wq, Wqk = heads * d, (heads + kv) * d
@@ -2626,7 +2629,7 @@ class WindowAttentionQkv(torch.autograd.Function):
     def backward(ctx, g):
         xs, qk, o, lse, qw, kw, positions, lengths = ctx.saved_tensors
         xb, xt, heads, kv, eps, rot, win = ctx.opts
-        gs, (gb, gt) = _strided(g)
+        gs, (gb, gt) = _strided(g, True)
         B, N, W = xs.shape
         d, es, dtc, dev = W // (heads + 2 * kv), xs.element_size(), _dt(xs), xs.device
         Wq, Wqk = heads * d, (heads + kv) * d
