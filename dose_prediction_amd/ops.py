@@ -8,6 +8,7 @@ Tensor conventions inside the HIP path
     consume packed copies cached per (parameter version, dtype).  Weight gradients are produced in fp32.
 PyTorch only provides device memory, the current stream and autograd bookkeeping here.
 """
+import functools
 import math
 import os
 
@@ -2338,7 +2339,7 @@ HEAD_DIMS = (32, 64, 96, 128)
 
 def _device_of(t):
     """Context in which launches go to t's device (nothing to do where it is the current one)."""
-    if _raw_device is not None and t.device.index == _raw_device():
+    if _raw_device is not None and t.get_device() == _raw_device():
         return _NO_GUARD
     return torch.cuda.device(t.device)
 
@@ -2358,11 +2359,12 @@ def _strided(t, tiles=False):
     """(tensor, strides of all but the last dimension): t itself where its last dimension is dense and every row 16-byte aligned (tiles: and
     its tokens, dimension 1, do not overlap and lie at most 16 MB apart), otherwise a contiguous copy."""
     st, es, shape = t.stride(), t.element_size(), t.shape
-    if t.is_contiguous() and t.data_ptr() % 16 == 0 and shape[-1] * es % 16 == 0:
-        return t, st[:-1]
-    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s * es % 16 == 0 for n, s in zip(shape[:-1], st))
-            and not (tiles and shape[1] > 1 and (st[1] < shape[-1] or st[1] * es > 1 << 24))):
-        return t, [0 if n <= 1 else s for n, s in zip(shape[:-1], st)]
+    if t.data_ptr() % 16 == 0 and (st[-1] == 1 or shape[-1] <= 1):
+        if t.is_contiguous() and st[-2] * es % 16 == 0 and t.numel():
+            return t, st[:-1]
+        if all(n <= 1 or s * es % 16 == 0 for n, s in zip(shape[:-1], st)) and not (
+                tiles and shape[1] > 1 and (st[1] < shape[-1] or st[1] * es > 1 << 24)):
+            return t, [0 if n <= 1 else s for n, s in zip(shape[:-1], st)]
     t = t.contiguous() if not t.is_contiguous() else t.clone()
     return t, t.stride()[:-1]
 
@@ -2376,39 +2378,48 @@ def _head_dim(width, heads, what):
     return d
 
 
+@functools.lru_cache(maxsize=256)
+def _rotary_plan(what, d, sections, base, interleaved):
+    """The part of the C ABI's arguments that depends on the configuration alone (checked once per configuration)."""
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * sum(sections) > d:
+        raise ValueError(f"{what}: sections {sections} of a head of {d} channels (1 to 4 axes, at most {d // 2} pairs)")
+    if not 1.0 < float(base) < 1e30:
+        raise ValueError(f"{what}: base {base}")
+    return (len(sections), *(int(n) for n in sections), *(0,) * (4 - len(sections)), float(base), int(bool(interleaved)))
+
+
+_NO_ROTARY = (0, 0, 0, 0, 0, 0, 0, 0.0, 0)
+
+
 def _rotary_args(what, x, d, positions, sections, base, interleaved):
     """(positions tensor, the C ABI's arguments behind the pointer) of a rotation; (None, ...) without one."""
     if positions is None:
         if sections is not None:
             raise ValueError(f"{what}: sections without positions")
-        return None, (0, 0, 0, 0, 0, 0, 0, 0.0, 0)
+        return None, _NO_ROTARY
     if sections is None:
         raise ValueError(f"{what}: positions need sections (rotated pairs of a head per axis)")
-    sections = tuple(int(s) for s in sections)
-    B, N = x.shape[:2]
-    if positions.dtype not in _POS_KIND:
+    plan = _rotary_plan(what, d, tuple(sections), base, interleaved)
+    B, N, shape, axes = x.shape[0], x.shape[1], positions.shape, plan[0]
+    kind = _POS_KIND.get(positions.dtype)
+    if kind is None:
         raise TypeError(f"{what}: positions are int32, int64 or float32, got {positions.dtype}")
     if positions.device != x.device:
         raise _lib.DoseHipError(f"{what}: positions on {positions.device}, rows on {x.device}")
-    if positions.dim() not in (2, 3) or positions.shape[-2:] != (N, len(sections)) or (positions.dim() == 3 and positions.shape[0] not in (1, B)):
-        raise ValueError(f"{what}: positions {tuple(positions.shape)} for {B} x {N} tokens and {len(sections)} axes")
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * sum(sections) > d:
-        raise ValueError(f"{what}: sections {sections} of a head of {d} channels (1 to 4 axes, at most {d // 2} pairs)")
-    if not 1.0 < float(base) < 1e30:
-        raise ValueError(f"{what}: base {base}")
-    positions = positions.contiguous()
-    posb = N * len(sections) if positions.dim() == 3 and positions.shape[0] == B else 0
-    return positions, (_POS_KIND[positions.dtype], posb, len(sections), *sections, *(0,) * (4 - len(sections)), float(base), int(bool(interleaved)))
+    if len(shape) not in (2, 3) or shape[-2] != N or shape[-1] != axes or (len(shape) == 3 and shape[0] not in (1, B)):
+        raise ValueError(f"{what}: positions {tuple(shape)} for {B} x {N} tokens and {axes} axes")
+    return positions.contiguous(), (kind, N * axes if len(shape) == 3 and shape[0] == B else 0, *plan)
 
 
-def _norm_weights(what, d, *ws):
-    out = []
+def _check_norm(what, d, *ws):
     for w in ws:
-        if w.dtype != torch.float32 or tuple(w.shape) != (d,):
+        if w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != d:
             raise ValueError(f"{what}: the norm's weights and biases are float32 [{d}], got {w.dtype} {tuple(w.shape)}")
-        w = w.detach().contiguous()
-        out.append(w if w.data_ptr() % 16 == 0 else w.clone())
-    return out
+
+
+def _dense(*ws):
+    """Weights as the kernels read them: dense, 16-byte aligned (themselves, as a rule)."""
+    return [w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.detach().clone(memory_format=torch.contiguous_format) for w in ws]
 
 
 class RotaryAxes(torch.autograd.Function):
@@ -2456,7 +2467,7 @@ class QkNormRotary(torch.autograd.Function):
         xs, (xb, xt) = _strided(x)
         B, N, W = x.shape
         d = W // (heads + kv)
-        qwd, qbd, kwd, kbd = _norm_weights("qk_norm_rotary", d, qw, qb, kw, kb)
+        qwd, qbd, kwd, kbd = _dense(qw, qb, kw, kb)
         y = torch.empty((B, N, W), dtype=x.dtype, device=x.device)
         with _device_of(x):
             _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, kv, d, _p(qwd), _p(qbd), _p(kwd), _p(kbd), eps,
@@ -2472,14 +2483,14 @@ class QkNormRotary(torch.autograd.Function):
         gs, (gb, gt) = _strided(g)
         B, N, W = g.shape
         d = W // (heads + kv)
-        qwd, kwd = _norm_weights("qk_norm_rotary", d, qw, kw)
+        qwd, kwd = _dense(qw, kw)
         gx = torch.empty((B, N, W), dtype=g.dtype, device=g.device)
         dw = torch.empty((4, d), dtype=torch.float32, device=g.device)
         part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=g.device)
         with _device_of(g):
             _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(gs), gb, gt, 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d, _p(qwd),
                       _p(kwd), eps, _p(positions), *rot, _dt(g), _stream())
-        return gx, dw[0], dw[1], dw[2], dw[3], None, None, None, None, None
+        return (gx, *dw.unbind(0), None, None, None, None, None)
 
 
 def qk_norm_rotary(x, heads, kv_heads, q_weight, q_bias, k_weight, k_bias, eps=1e-5, positions=None, sections=None, base=10000.0,
@@ -2492,7 +2503,7 @@ def qk_norm_rotary(x, heads, kv_heads, q_weight, q_bias, k_weight, k_bias, eps=1
     if x.dim() != 3 or heads < 1 or kv_heads < 1:
         raise ValueError(f"{what}: x is [B, N, channels] with heads and kv_heads of at least 1, got {tuple(x.shape)}, {heads}, {kv_heads}")
     d = _head_dim(x.shape[-1], heads + kv_heads, what)
-    _norm_weights(what, d, q_weight, q_bias, k_weight, k_bias)
+    _check_norm(what, d, q_weight, q_bias, k_weight, k_bias)
     positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
     _chk_dev(x, q_weight, q_bias, k_weight, k_bias)
     return QkNormRotary.apply(x, q_weight, q_bias, k_weight, k_bias, int(heads), int(kv_heads), float(eps), positions, rot)
@@ -2613,7 +2624,7 @@ class WindowAttentionQkv(torch.autograd.Function):
         with _device_of(qkv):
             qk, qkb, qkt = xs, xb, xt
             if pre:
-                ws4 = _norm_weights("window_attention_qkv", d, qw, qb, kw, kb) if qw is not None else (None,) * 4
+                ws4 = _dense(qw, qb, kw, kb) if qw is not None else (None,) * 4
                 qk, qkb, qkt = torch.empty((B, N, Wqk), dtype=qkv.dtype, device=qkv.device), N * Wqk, Wqk
                 _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(qk), qkb, qkt, B, N, heads, kv, d, *(_p(w) for w in ws4), eps, _p(positions), *rot,
                           0, dtc, _stream())
@@ -2648,12 +2659,12 @@ class WindowAttentionQkv(torch.autograd.Function):
             if qk is not None:
                 part = None
                 if qw is not None:
-                    qw, kw = _norm_weights("window_attention_qkv", d, qw, kw)
+                    qw, kw = _dense(qw, kw)
                     dw = torch.empty((4, d), dtype=torch.float32, device=dev)
                     part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=dev)
                 _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d,
                           _p(qw), _p(kw), eps, _p(positions), *rot, dtc, _stream())
-        return (gx, *((dw[0], dw[1], dw[2], dw[3]) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
+        return (gx, *(dw.unbind(0) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
 
 
 def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks=0, lengths=None, scale=None, norm=None, eps=1e-5,
@@ -2671,7 +2682,7 @@ def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks
         raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
     d = _head_dim(qkv.shape[-1], heads + 2 * kv, what)
     if norm[0] is not None:
-        _norm_weights(what, d, *norm)
+        _check_norm(what, d, *norm)
     positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
     win = _window_args(what, left, right, sinks, scale, d)
     lengths = _per_sequence(what, "lengths", lengths, qkv.shape[0], qkv)
