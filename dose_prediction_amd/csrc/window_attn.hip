@@ -185,9 +185,9 @@ template <typename T, int D> struct Frags {
 // Waves per SIMD that the register budget is cut for.  Two (256 registers) also keep the matrix accumulators in plain VGPRs: with more the
 // compiler puts them into AGPRs and copies them back and forth around every rescale and mask (24 instead of 9 vector instructions per
 // matrix instruction in the forward kernel).  One where two would spill.
-template <typename T, int D> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
+template <typename T, int D, bool WIDE> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : sizeof(T) == 2 && D == 128 && WIDE ? 3 : 2; }
 template <typename T, int D> constexpr int waves_dq() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
-template <typename T, int D> constexpr int waves_kv() { return D >= 96 || (sizeof(T) == 4 && D >= 64) ? 1 : 2; }
+template <typename T, int D> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : 2; }
 
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
@@ -216,7 +216,8 @@ template <typename T, int D, bool WIDE> struct Shape {
   using C = Cfg<T, D>;
   // WIDE: four waves own 32 rows each and share every staged tile (one barrier per tile).  Otherwise all four own the same 32 rows, stream
   // different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
-  static constexpr int KS = (WIDE && C::ES == 2) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64;
+  // (heads of 128: 32-key tiles and 168 registers, so that three blocks stay on a CU instead of two: 172 -> 156 us at 6 heads, window 1152)
+  static constexpr int KS = (WIDE && C::ES == 2 && D < 128) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64;
   // tiles in LDS per stream: the next one arrives while one is worked on (narrow: where two still leave room for two blocks on a CU)
   static constexpr int NBUF = WIDE || (C::ES == 2 && D <= 64) ? 2 : 1;
   static constexpr int tile = KT * C::PITCH, sets = (WIDE ? 1 : 4) * NBUF, stage = sets * 2 * tile;
@@ -225,7 +226,9 @@ template <typename T, int D, bool WIDE> struct Shape {
   static constexpr int fwd = big + (WIDE ? 0 : 2 * 4 * 32 * 4);
   // dK / dV: tiles of RT query rows and of the output's gradient, their lse and delta behind all tiles
   static constexpr int RS = (WIDE && C::ES == 2 && D < 128) ? 2 : 1, RT = 32 * RS, rtile = RT * C::PITCH, rstage = sets * 2 * rtile;
-  static constexpr int kv_all = rstage + sets * 512, kvb = kv_all > merge ? kv_all : merge;
+  // heads of 128 in 16 bits: the owned keys' values wait in LDS too, not in registers (two waves per SIMD instead of one)
+  static constexpr bool VLDS = C::ES == 2 && D == 128;
+  static constexpr int vals = rstage + sets * 512, kv_all = vals + (VLDS ? ROWS * C::PITCH : 0), kvb = kv_all > merge ? kv_all : merge;
   static_assert(fwd <= 160 * 1024 && kvb <= 160 * 1024, "LDS of a CU");
 };
 
@@ -270,20 +273,21 @@ struct Rows {
 // Loads of the prologue are waited for before the loop: otherwise the waits for them sit inside it and hold up the copies instead.
 #define PROLOGUE_LOADED __builtin_amdgcn_s_waitcnt(0)
 
-// s += X x, t += Y y over the head dimension: 32 rows from r0 on of two staged tiles against fragments in registers
-template <typename T, int D>
-__device__ __forceinline__ void two_products(const Frags<T, D>& F, const char* x0, const char* y0, int r0, const Frag8<T>* x, const Frag8<T>* y, v16f& s, v16f& t) {
-  constexpr int KK = Cfg<T, D>::KK, G = sizeof(T) == 4 ? 1 : KK < 4 ? KK : KK == 6 ? 3 : 4;
+// s += X x, t += Y y over the head dimension: 32 rows from r0 on of two staged tiles against fragments x[k], y(k)
+template <typename T, int D, int G, typename Y>
+__device__ __forceinline__ void two_products(const Frags<T, D>& F, const char* x0, const char* y0, int r0, const Frag8<T>* x, Y y, v16f& s, v16f& t) {
 #pragma unroll
-  for (int g = 0; g < KK; g += G) {
-    Frag8<T> xf[G], yf[G];
+  for (int g = 0; g < Cfg<T, D>::KK; g += G) {
+    Frag8<T> xf[G], yf[G], yr[G];
 #pragma unroll
-    for (int i = 0; i < G; i++) { xf[i] = F.rows(x0, r0, g + i); yf[i] = F.rows(y0, r0, g + i); }
+    for (int i = 0; i < G; i++) { xf[i] = F.rows(x0, r0, g + i); yf[i] = F.rows(y0, r0, g + i); yr[i] = y(g + i); }
     READS_FIRST;
 #pragma unroll
-    for (int i = 0; i < G; i++) { s = mma32(xf[i], x[g + i], s); t = mma32(yf[i], y[g + i], t); }
+    for (int i = 0; i < G; i++) { s = mma32(xf[i], x[g + i], s); t = mma32(yf[i], yr[i], t); }
   }
 }
+// k steps whose operands are read together (an fp32 operand is twice the registers)
+template <typename T, int D> constexpr int read_group() { return sizeof(T) == 4 ? 1 : D == 32 ? 2 : D == 96 ? 3 : 4; }
 
 // scores of keys k0 .. k0 + 31 that the lane's row does not see -> `none`.  Behind the sinks a seen key is one range: one subtraction and one
 // unsigned comparison a key.  (A row that is not live may keep any value: its column is thrown away.)
@@ -338,7 +342,7 @@ template <typename T> __device__ __forceinline__ void st4_grad(void* p, int64_t 
 
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, (waves_fwd<T, D>())) void k_win_fwd(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D>())) void k_win_fwd(const WinA
     if (wave.none(a, k0)) return;
     v16f s = zero16();
     {
-      constexpr int G = C::KK == 6 ? 3 : C::KK < 4 ? C::KK : 4;
+      constexpr int G = C::KK == 6 ? 3 : C::KK == 4 ? 4 : 2;
 #pragma unroll
       for (int g = 0; g < C::KK; g += G) {
         Frag8<T> kf[G];
@@ -565,7 +569,7 @@ __global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArg
   auto step = [&](const char* ks, const char* vs, int u, int k0) {
     if (wave.none(a, k0)) return;
     v16f s = zero16(), dp = zero16();
-    two_products<T, D>(F, ks, vs, 32 * u, qf, gf, s, dp);
+    two_products<T, D, read_group<T, D>()>(F, ks, vs, 32 * u, qf, [&](int k) { return gf[k]; }, s, dp);
     Frag8<T> kt[2][C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; dt++) kt[0][dt] = F.cols(ks, 32 * u, dt);
@@ -677,13 +681,20 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   const T* Qb = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)kvh * a.group * a.q.h;
   const T* Gb = (const T*)a.go.p + (int64_t)b * a.go.b + (int64_t)kvh * a.group * a.go.h;
   const float *lseb = a.lse + (int64_t)bh * a.rows, *dlb = a.delta + (int64_t)bh * a.rows;
-  Frag8<T> kf[C::KK], vf[C::KK];
+  const Frags<T, D> F(lane);
+  char* const vals = smem + S::vals + (WIDE ? wv * 32 * C::PITCH : 0);
+  Frag8<T> kf[C::KK], vf[S::VLDS ? 1 : C::KK];
   {
     const int jc = live ? j : 0;       // (a key behind the sequence: any key, its column is thrown away)
     const T* Kr = (const T*)a.k.p + (int64_t)b * a.k.b + (int64_t)jc * a.k.t + (int64_t)kvh * a.k.h;
     const T* Vr = (const T*)a.v.p + (int64_t)b * a.v.b + (int64_t)jc * a.v.t + (int64_t)kvh * a.v.h;
 #pragma unroll
-    for (int kk = 0; kk < C::KK; kk++) { kf[kk] = ldg8(Kr + 16 * kk + 8 * h); vf[kk] = ldg8(Vr + 16 * kk + 8 * h); }
+    for (int kk = 0; kk < C::KK; kk++) {
+      kf[kk] = ldg8(Kr + 16 * kk + 8 * h);
+      // (narrow: the four waves own the same keys and write the same values; a wave reads behind its own writes)
+      if constexpr (S::VLDS) *(v4u*)(vals + F.row + (((2 * kk) ^ F.fx) << 4)) = ldg8(Vr + 16 * kk + 8 * h).u;
+      else vf[kk] = ldg8(Vr + 16 * kk + 8 * h);
+    }
   }
   v16f ak[C::DT], av[C::DT];
 #pragma unroll
@@ -702,15 +713,17 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   // tiles of RT tokens of one query head, the heads of the group one after the other
   const int per_head = (block.hi - block.lo + S::RT - 1) / S::RT, ntile = per_head * a.group;
   const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t0 = chunk * per, t1 = min(ntile, t0 + per);
-  const Frags<T, D> F(lane);
 
   auto step = [&](const char* qs, const char* gs, const float* sl, const float* sd, int u, int i0) {      // 32 query rows, i0 the first token
     if (i0 >= any_hi || i0 + 32 <= any_lo) return;
     v16f s = zero16(), dp = zero16();
-    two_products<T, D>(F, qs, gs, 32 * u, kf, vf, s, dp);
+    if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return F.rows(vals, 0, k); }, s, dp);
+    else two_products<T, D, read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
+    // (heads of 96 and 128: no registers to read the k-major operands ahead)
+    constexpr int AH = C::ES == 2 && D >= 96 ? 0 : C::DT;
     Frag8<T> gt[C::DT], qt[C::DT];
 #pragma unroll
-    for (int dt = 0; dt < C::DT; dt++) { gt[dt] = F.cols(gs, 32 * u, dt); qt[dt] = F.cols(qs, 32 * u, dt); }
+    for (int dt = 0; dt < AH; dt++) { gt[dt] = F.cols(gs, 32 * u, dt); qt[dt] = F.cols(qs, 32 * u, dt); }
     READS_FIRST;
     mma_ready<T>(s, dp);
     if (!(i0 >= all_lo && i0 + 32 <= all_hi)) {
@@ -738,14 +751,15 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
       Frag8<T> gn[C::DT], qn[C::DT];
       if (st == 0) {
 #pragma unroll
-        for (int dt = 0; dt < C::DT; dt++) { gn[dt] = F.cols(gs, 32 * u + 16, dt); qn[dt] = F.cols(qs, 32 * u + 16, dt); }
+        for (int dt = 0; dt < AH; dt++) { gn[dt] = F.cols(gs, 32 * u + 16, dt); qn[dt] = F.cols(qs, 32 * u + 16, dt); }
         READS_FIRST;
       }
 #pragma unroll
       for (int dt = 0; dt < C::DT; dt++) {
+        if (!AH) { gt[dt] = F.cols(gs, 32 * u + 16 * st, dt); qt[dt] = F.cols(qs, 32 * u + 16 * st, dt); }
         av[dt] = mma32(gt[dt], pf, av[dt]);
         ak[dt] = mma32(qt[dt], df, ak[dt]);
-        if (st == 0) { gt[dt] = gn[dt]; qt[dt] = qn[dt]; }
+        if (AH && st == 0) { gt[dt] = gn[dt]; qt[dt] = qn[dt]; }
       }
     }
   };
@@ -872,7 +886,7 @@ Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right
   p.sink_tiles = 0; p.nchunk = 1;
   if (sinks > 0 && left < FAR && Nk > 0) {
     const int64_t usual = ((int64_t)left + (right >= FAR ? Nk : right) + kb) * group;      // rows of any other tile
-    int64_t n = rows / (usual < 512 ? 512 : usual);
+    int64_t n = rows / (usual < 128 ? 128 : usual);
     const int64_t st = ((sinks < Nk ? sinks : Nk) + kb - 1) / kb, most = (64ll << 20) / (bk * st * 2 * kb * d);      // (256 MB of partial sums at most)
     if (n > most) n = most;
     p.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
