@@ -8,8 +8,8 @@
 //
 // Bound: HBM.  A value is read once and written once (the backward pass reads x and gy, writes gx; the row statistics are recomputed from
 // the x that is in registers anyway, so nothing but x is kept between the passes).
-// Split: a lane owns 8 PAIRS of one head (16 channels), so that a turn needs no other lane and a head is d / 16 lanes whose three sums are
-// two or three shuffles.  Cosines and sines belong to a token, not to a head: a block computes those of its tokens once into LDS and all
+// Split: a lane owns 8 PAIRS of one head (16 channels, whole 16-byte pieces next to its neighbours'), so that a turn needs no other lane and a
+// head is d / 16 lanes whose sums are two or three shuffles.  Cosines and sines belong to a token, not to a head: a block computes those of its tokens once into LDS and all
 // heads of q and k share them.  Angles are formed in 64 bits (position * frequency, reduced to a fraction of a turn) because a far position
 // times a frequency has no fraction left in 32.
 #include "common.h"
@@ -36,55 +36,82 @@ struct QkArgs {
   int64_t N, tokens;
 };
 
-template <typename T> __device__ __forceinline__ void ld8(const T* p, float* v);
-template <> __device__ __forceinline__ void ld8<float>(const float* p, float* v) {
-  const v4f a = *(const v4f*)p, b = *(const v4f*)(p + 4);
+// 16 bytes
+template <typename T> __device__ __forceinline__ void ld_piece(const T* p, float* v);
+template <> __device__ __forceinline__ void ld_piece<float>(const float* p, float* v) {
+  const v4f a = *(const v4f*)p;
 #pragma unroll
-  for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
+  for (int i = 0; i < 4; i++) v[i] = a[i];
 }
-template <> __device__ __forceinline__ void ld8<bf16_t>(const bf16_t* p, float* v) {
+template <> __device__ __forceinline__ void ld_piece<bf16_t>(const bf16_t* p, float* v) {
   const v4u u = *(const v4u*)p;
 #pragma unroll
   for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
 }
-template <> __device__ __forceinline__ void ld8<f16_t>(const f16_t* p, float* v) {
+template <> __device__ __forceinline__ void ld_piece<f16_t>(const f16_t* p, float* v) {
   const v8h u = *(const v8h*)p;
 #pragma unroll
   for (int i = 0; i < 8; i++) v[i] = (float)u[i];
 }
-template <typename T> __device__ __forceinline__ void st8(T* p, const float* v);
-template <> __device__ __forceinline__ void st8<float>(float* p, const float* v) {
-  *(v4f*)p = (v4f){v[0], v[1], v[2], v[3]};
-  *(v4f*)(p + 4) = (v4f){v[4], v[5], v[6], v[7]};
-}
-template <> __device__ __forceinline__ void st8<bf16_t>(bf16_t* p, const float* v) {
+template <typename T> __device__ __forceinline__ void st_piece(T* p, const float* v);
+template <> __device__ __forceinline__ void st_piece<float>(float* p, const float* v) { *(v4f*)p = (v4f){v[0], v[1], v[2], v[3]}; }
+template <> __device__ __forceinline__ void st_piece<bf16_t>(bf16_t* p, const float* v) {
   v4u u;
 #pragma unroll
   for (int i = 0; i < 4; i++) u[i] = (unsigned)f2bf(v[2 * i]) | ((unsigned)f2bf(v[2 * i + 1]) << 16);
   *(v4u*)p = u;
 }
-template <> __device__ __forceinline__ void st8<f16_t>(f16_t* p, const float* v) {
+template <> __device__ __forceinline__ void st_piece<f16_t>(f16_t* p, const float* v) {
   v8h u;
 #pragma unroll
   for (int i = 0; i < 8; i++) u[i] = (f16_t)v[i];
   *(v8h*)p = u;
 }
 
-// the 16 channels of lane c of a head: v[e] and v[8 + e] are the two members of pair 8 c + e
-template <typename T, int D> __device__ __forceinline__ void load_pairs(const T* p, int c, int inter, float* v) {
-  if (!inter) { ld8(p + 8 * c, v); ld8(p + D / 2 + 8 * c, v + 8); return; }
-  float t[16];
-  ld8(p + 16 * c, t); ld8(p + 16 * c + 8, t + 8);
+template <int D> struct Lanes { static constexpr int LG = D / 16, LGP = D == 96 ? 8 : D / 16; };
+
+// Which of a head's D / 2 pairs lane c owns: 16-byte pieces c, c + LG, c + 2 LG ..., so that the lanes of a head read consecutive pieces and
+// the two members of a pair are both the lane's own (8 consecutive channels per lane instead: 33 -> 21 us forward, 53 -> 37 us backward for fp32
+// rows of 16 heads of 64, 13 801 tokens).  PW pairs come with a piece (of each half of the head, or, interleaved, inside it); all types of one
+// kernel use the ownership of the storage type T.
+template <typename T, int D, bool IN> struct Own {
+  static constexpr int EPP = 16 / (int)sizeof(T), PW = IN ? EPP / 2 : EPP, LG = Lanes<D>::LG;
+  __device__ __forceinline__ static int pair(int c, int e) { return PW * (c + LG * (e / PW)) + e % PW; }
+  __device__ __forceinline__ static int chan(int c, int k) {      // channel of v[k]: k < 8 the first members of the pairs, then the second
+    const int p = pair(c, k & 7);
+    return IN ? 2 * p + (k >> 3) : p + (k >> 3) * (D / 2);
+  }
+  // the lane's 16 channels of a row of U (U = T: whole pieces; a wider U: what lies in a piece of T, in pieces of its own)
+  template <typename U> __device__ __forceinline__ static void load(const U* p, int c, float* v) {
+    constexpr int UP = 16 / (int)sizeof(U), R = sizeof(U) / sizeof(T) > 0 ? EPP / UP : 1;
+    static_assert(UP <= EPP, "");
 #pragma unroll
-  for (int e = 0; e < 8; e++) { v[e] = t[2 * e]; v[8 + e] = t[2 * e + 1]; }
-}
-template <typename T, int D> __device__ __forceinline__ void store_pairs(T* p, int c, int inter, const float* v) {
-  if (!inter) { st8(p + 8 * c, v); st8(p + D / 2 + 8 * c, v + 8); return; }
-  float t[16];
+    for (int k = 0; k < 16 / EPP; k++) {
+      float t[EPP];
+      // half layout: the first 8 / EPP pieces from the first half of the head, the others from the second
+      const int piece = IN ? c + LG * k : c + LG * (k % (8 / EPP)), base = IN ? 0 : (k / (8 / EPP)) * (D / 2);
 #pragma unroll
-  for (int e = 0; e < 8; e++) { t[2 * e] = v[e]; t[2 * e + 1] = v[8 + e]; }
-  st8(p + 16 * c, t); st8(p + 16 * c + 8, t + 8);
-}
+      for (int r = 0; r < R; r++) ld_piece(p + base + piece * EPP + r * UP, t + r * UP);
+      put(t, k, v);
+    }
+  }
+  __device__ __forceinline__ static void store(T* p, int c, const float* v) {
+#pragma unroll
+    for (int k = 0; k < 16 / EPP; k++) {
+      float t[EPP];
+      const int piece = IN ? c + LG * k : c + LG * (k % (8 / EPP)), base = IN ? 0 : (k / (8 / EPP)) * (D / 2);
+#pragma unroll
+      for (int i = 0; i < EPP; i++) t[i] = IN ? v[(k * (EPP / 2) + i / 2) + 8 * (i & 1)] : v[k * EPP + i];
+      st_piece(p + base + piece * EPP, t);
+    }
+  }
+  __device__ __forceinline__ static void put(const float* t, int k, float* v) {
+#pragma unroll
+    for (int i = 0; i < EPP; i++) {
+      if (IN) v[(k * (EPP / 2) + i / 2) + 8 * (i & 1)] = t[i]; else v[k * EPP + i] = t[i];
+    }
+  }
+};
 
 template <int LGP> __device__ __forceinline__ float head_sum(float v) {
 #pragma unroll
@@ -115,8 +142,6 @@ template <int D> __device__ __forceinline__ void fill_angles(const RotPlan& R, i
   }
 }
 
-template <int D> struct Lanes { static constexpr int LG = D / 16, LGP = D == 96 ? 8 : D / 16; };
-
 template <int D> __device__ __forceinline__ void head_stats(const float* v, bool on, float eps, float& mean, float& rstd) {
   float s = 0.f;
 #pragma unroll
@@ -128,9 +153,10 @@ template <int D> __device__ __forceinline__ void head_stats(const float* v, bool
   rstd = 1.f / sqrtf(head_sum<Lanes<D>::LGP>(on ? q : 0.f) * (1.f / D) + eps);
 }
 
-template <typename T, int D, bool NORM>
+template <typename T, int D, bool NORM, bool IN>
 __global__ void __launch_bounds__(256) k_qk_rotary_fwd(const QkArgs a, const RotPlan R) {
   constexpr int LG = Lanes<D>::LG, LGP = Lanes<D>::LGP;
+  using O = Own<T, D, IN>;
   extern __shared__ __attribute__((aligned(16))) float2 cs[];
   const int64_t t0 = (int64_t)blockIdx.x * a.tok, b0 = t0 / a.N, r0 = t0 - b0 * a.N;
   const int n = (int)min((int64_t)a.tok, a.tokens - t0), c = threadIdx.x % LGP;
@@ -140,13 +166,13 @@ __global__ void __launch_bounds__(256) k_qk_rotary_fwd(const QkArgs a, const Rot
   for (int part = 0; part < 2; part++) {
     const int heads = part ? a.hk : a.hq;
     float w[16], bi[16];
-    if (NORM && on && heads) { load_pairs<float, D>(part ? a.wk : a.wq, c, R.interleaved, w); load_pairs<float, D>(part ? a.bk : a.bq, c, R.interleaved, bi); }
+    if (NORM && on && heads) { O::load(part ? a.wk : a.wq, c, w); O::load(part ? a.bk : a.bq, c, bi); }
     for (int i = threadIdx.x / LGP; i < n * heads; i += 256 / LGP) {
       const int t = i / heads, h = i - t * heads + (part ? a.hq : 0);
       int64_t b, r;
       locate(a.N, b0, r0, t, b, r);
       float v[16];
-      if (on) load_pairs<T, D>((const T*)a.x + b * a.xb + r * a.xt + h * D, c, R.interleaved, v);
+      if (on) O::load((const T*)a.x + b * a.xb + r * a.xt + h * D, c, v);
       if (NORM) {
         float mean, rstd;
         head_stats<D>(v, on, a.eps, mean, rstd);
@@ -154,23 +180,24 @@ __global__ void __launch_bounds__(256) k_qk_rotary_fwd(const QkArgs a, const Rot
         for (int e = 0; e < 16; e++) v[e] = (v[e] - mean) * rstd * w[e] + bi[e];
       }
       if (R.pairs && on) {
-        const float2* q = cs + t * (D / 2) + 8 * c;
+        const float2* q = cs + t * (D / 2);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const float2 z = q[e];
+          const float2 z = q[O::pair(c, e)];
           const float x0 = v[e], x1 = v[8 + e];
           v[e] = fmaf(x0, z.x, -(x1 * z.y)); v[8 + e] = fmaf(x0, z.y, x1 * z.x);
         }
       }
-      if (on) store_pairs<T, D>((T*)a.y + b * a.yb + r * a.yt + h * D, c, R.interleaved, v);
+      if (on) O::store((T*)a.y + b * a.yb + r * a.yt + h * D, c, v);
     }
   }
 }
 
 // G: type of the incoming gradient (fp32 where the attention's backward pass keeps the gradient of q and k unrounded for this kernel)
-template <typename T, typename G, int D, bool NORM>
+template <typename T, typename G, int D, bool NORM, bool IN>
 __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const RotPlan R) {
   constexpr int LG = Lanes<D>::LG, LGP = Lanes<D>::LGP;
+  using O = Own<T, D, IN>;
   extern __shared__ __attribute__((aligned(16))) float2 cs[];
   const int c = threadIdx.x % LGP;
   const bool on = c < LG;
@@ -188,21 +215,21 @@ __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const Rot
     for (int part = 0; part < 2; part++) {
       const int heads = part ? a.hk : a.hq;
       float w[16];
-      if (NORM && on && heads) load_pairs<float, D>(part ? a.wk : a.wq, c, R.interleaved, w);
+      if (NORM && on && heads) O::load(part ? a.wk : a.wq, c, w);
       for (int i = threadIdx.x / LGP; i < n * heads; i += 256 / LGP) {
         const int t = i / heads, h = i - t * heads + (part ? a.hq : 0);
         int64_t b, r;
         locate(a.N, b0, r0, t, b, r);
         float g[16], v[16];
         if (on) {
-          load_pairs<G, D>((const G*)a.g + b * a.gb + r * a.gt + h * D, c, R.interleaved, g);
-          if (NORM) load_pairs<T, D>((const T*)a.x + b * a.xb + r * a.xt + h * D, c, R.interleaved, v);
+          O::load((const G*)a.g + b * a.gb + r * a.gt + h * D, c, g);
+          if (NORM) O::load((const T*)a.x + b * a.xb + r * a.xt + h * D, c, v);
         }
         if (R.pairs && on) {
-          const float2* q = cs + t * (D / 2) + 8 * c;
+          const float2* q = cs + t * (D / 2);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            const float2 z = q[e];
+            const float2 z = q[O::pair(c, e)];
             const float g0 = g[e], g1 = g[8 + e];
             g[e] = fmaf(g0, z.x, -(g1 * z.y)); g[8 + e] = fmaf(g0, z.y, g1 * z.x);
           }
@@ -223,7 +250,7 @@ __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const Rot
 #pragma unroll
           for (int e = 0; e < 16; e++) g[e] = rstd * (g[e] - s1 - v[e] * s2);
         }
-        if (on) store_pairs<T, D>((T*)a.y + b * a.yb + r * a.yt + h * D, c, R.interleaved, g);
+        if (on) O::store((T*)a.y + b * a.yb + r * a.yt + h * D, c, g);
       }
     }
   }
@@ -237,7 +264,7 @@ __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const Rot
         float s = dw[p][e], u = db[p][e];
 #pragma unroll
         for (int o = 32; o >= LGP; o >>= 1) { s += __shfl_xor(s, o, 64); u += __shfl_xor(u, o, 64); }
-        const int ch = R.interleaved ? 16 * c + 2 * (e & 7) + (e >> 3) : 8 * c + (e & 7) + (e >> 3) * (D / 2);
+        const int ch = O::chan(c, e);
         if (lane < LGP && on) { red[wv][2 * p][ch] = s; red[wv][2 * p + 1][ch] = u; }
       }
     __syncthreads();
@@ -281,7 +308,20 @@ int make_plan(const char* name, RotPlan& R, const void* pos, int pos_kind, int64
   for (int ax = 0; ax < naxes; ax++) {
     if (sec[ax] < 0 || sec[ax] > d / 2) DP_FAIL("%s: %d pairs for axis %d of a head of %d", name, sec[ax], ax, d);
     if (R.pairs + sec[ax] > d / 2) DP_FAIL("%s: more rotated pairs than a head of %d has", name, d);
-    for (int e = 0; e < sec[ax]; e++) { R.freq[R.pairs] = pow(base, -(double)e / sec[ax]) / 6.283185307179586476925287; R.axis[R.pairs++] = ax; }
+    R.pairs += sec[ax];
+  }
+  // (64 powers are 3 us of host time: the table of the configuration that this thread used last is kept)
+  static thread_local struct { double base; int sec[4]; int naxes; double freq[MAXPAIRS]; int axis[MAXPAIRS]; } kept = {0.0, {0, 0, 0, 0}, 0, {}, {}};
+  bool same = kept.base == base && kept.naxes == naxes;
+  for (int ax = 0; ax < naxes && same; ax++) same = kept.sec[ax] == sec[ax];
+  if (!same) {
+    int n = 0;
+    for (int ax = 0; ax < naxes; ax++)
+      for (int e = 0; e < sec[ax]; e++) { kept.freq[n] = pow(base, -(double)e / sec[ax]) / 6.283185307179586476925287; kept.axis[n++] = ax; }
+    for (int ax = 0; ax < 4; ax++) kept.sec[ax] = ax < naxes ? sec[ax] : 0;
+    kept.base = base; kept.naxes = naxes;
+  }
+  for (int i = 0; i < R.pairs; i++) { R.freq[i] = kept.freq[i]; R.axis[i] = kept.axis[i];
   }
   return 0;
 }
@@ -299,6 +339,8 @@ int block_tokens(int64_t tokens) { return tokens >= 8192 ? 8 : tokens >= 2048 ? 
 
 #define QK_DIMS(d, ...) do { if ((d) == 32) { constexpr int D = 32; __VA_ARGS__; } else if ((d) == 64) { constexpr int D = 64; __VA_ARGS__; } \
     else if ((d) == 96) { constexpr int D = 96; __VA_ARGS__; } else { constexpr int D = 128; __VA_ARGS__; } } while (0)
+
+#define QK_IN(in, ...) do { if (in) { constexpr bool IN = true; __VA_ARGS__; } else { constexpr bool IN = false; __VA_ARGS__; } } while (0)
 
 extern "C" int dp_qk_rotary_parts(int64_t tokens) {
   const int64_t nblk = (tokens + block_tokens(tokens) - 1) / block_tokens(tokens);
@@ -326,8 +368,8 @@ extern "C" int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, 
   QkArgs a{x, nullptr, y, xb, xt, 0, 0, yb, yt, wq, bq, wk, bk, nullptr, eps, inverse ? -1.f : 1.f, heads, kv_heads, tok, N, tokens};
   const size_t smem = R.pairs ? (size_t)tok * (d / 2) * sizeof(float2) : 0;
   const dim3 grid((unsigned)((tokens + tok - 1) / tok));
-  DP_DISPATCH(dtype, QK_DIMS(d, if (norm) hipLaunchKernelGGL((k_qk_rotary_fwd<T, D, true>), grid, dim3(256), smem, STREAM, a, R);
-                                else hipLaunchKernelGGL((k_qk_rotary_fwd<T, D, false>), grid, dim3(256), smem, STREAM, a, R)));
+  DP_DISPATCH(dtype, QK_DIMS(d, QK_IN(R.interleaved, if (norm) hipLaunchKernelGGL((k_qk_rotary_fwd<T, D, true, IN>), grid, dim3(256), smem, STREAM, a, R);
+                                                      else hipLaunchKernelGGL((k_qk_rotary_fwd<T, D, false, IN>), grid, dim3(256), smem, STREAM, a, R))));
   DP_CHECK_LAUNCH("qk_rotary_fwd"); return 0;
 }
 
@@ -356,8 +398,9 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
   QkArgs a{x, g, gx, xb, xt, gb, gt, gxb, gxt, wq, nullptr, wk, nullptr, part, eps, 1.f, heads, kv_heads, tok, N, tokens};
   const size_t smem = R.pairs ? (size_t)tok * (d / 2) * sizeof(float2) : 0;
   const int nblk = norm ? dp_qk_rotary_parts(tokens) : (int)((tokens + tok - 1) / tok);
-#define QK_BWD(TG) DP_DISPATCH(dtype, QK_DIMS(d, if (norm) hipLaunchKernelGGL((k_qk_rotary_bwd<T, TG, D, true>), dim3(nblk), dim3(256), smem, STREAM, a, R); \
-                                                 else hipLaunchKernelGGL((k_qk_rotary_bwd<T, TG, D, false>), dim3(nblk), dim3(256), smem, STREAM, a, R)))
+#define QK_BWD(TG) DP_DISPATCH(dtype, QK_DIMS(d, QK_IN(R.interleaved, \
+    if (norm) hipLaunchKernelGGL((k_qk_rotary_bwd<T, TG, D, true, IN>), dim3(nblk), dim3(256), smem, STREAM, a, R); \
+    else hipLaunchKernelGGL((k_qk_rotary_bwd<T, TG, D, false, IN>), dim3(nblk), dim3(256), smem, STREAM, a, R))))
   if (g_f32) QK_BWD(float); else QK_BWD(T);
   DP_CHECK_LAUNCH("qk_rotary_bwd");
   if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 32)), dim3(1024), 0, STREAM, (const float*)part, dw, nblk, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd(dw)"); }

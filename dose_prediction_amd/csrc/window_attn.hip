@@ -13,6 +13,7 @@
 // row's scores, and the accumulator registers are, pair by pair of 8-row groups, the B operand of the second product; its A operand is
 // the streamed tile read k-major from LDS (ds_read_b64_tr_b16).  Running maximum and sum are one register per lane, fp32.
 #include "common.h"
+#include <atomic>
 
 #define STREAM ((hipStream_t)stream)
 
@@ -857,11 +858,15 @@ __global__ __launch_bounds__(256) void k_win_sink_sum(const WinArgs a, int keys)
 }
 
 // ------------------------------------------------------------------------------------------------ host
-int raise_lds(const void* kern, size_t smem, const char* name) {
-  if (smem > 48 * 1024) {
-    hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != hipSuccess) { (void)hipGetLastError(); DP_FAIL("%s: cannot raise dynamic LDS to %zu: %s", name, smem, hipGetErrorString(e)); }
-  }
+// (`done`: a bit per device on which this kernel's limit has been raised)
+int raise_lds(const void* kern, size_t smem, const char* name, std::atomic<uint64_t>& done) {
+  if (smem <= 48 * 1024) return 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 64;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return 0;
+  hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != hipSuccess) { (void)hipGetLastError(); DP_FAIL("%s: cannot raise dynamic LDS to %zu: %s", name, smem, hipGetErrorString(e)); }
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return 0;
 }
 
@@ -917,7 +922,8 @@ template <typename T, int D, bool WIDE> int run_fwd(const WinArgs& a, int B, hip
   auto kern = k_win_fwd<T, D, WIDE>;
   constexpr size_t smem = Shape<T, D, WIDE>::fwd;
   static_assert(smem <= 160 * 1024, "LDS of a CU");
-  if (raise_lds((const void*)kern, smem, "window_attention_fwd")) return 1;
+  static std::atomic<uint64_t> done{0};
+  if (raise_lds((const void*)kern, smem, "window_attention_fwd", done)) return 1;
   hipLaunchKernelGGL(kern, dim3(a.tiles * a.nsplit * B * a.kv), dim3(256), smem, st, a);
   DP_CHECK_LAUNCH("window_attention_fwd");
   if (a.nsplit > 1) {
@@ -929,7 +935,8 @@ template <typename T, int D, bool WIDE> int run_fwd(const WinArgs& a, int B, hip
 template <typename T, int D, bool WIDE> int run_dq(const WinArgs& a, int B, hipStream_t st) {
   auto kern = k_win_dq<T, D, WIDE>;
   constexpr size_t smem = Shape<T, D, WIDE>::big;
-  if (raise_lds((const void*)kern, smem, "window_attention_bwd")) return 1;
+  static std::atomic<uint64_t> done{0};
+  if (raise_lds((const void*)kern, smem, "window_attention_bwd", done)) return 1;
   hipLaunchKernelGGL(kern, dim3(a.tiles * B * a.kv), dim3(256), smem, st, a);
   DP_CHECK_LAUNCH("window_attention_bwd(dq)");
   return 0;
@@ -938,7 +945,8 @@ template <typename T, int D, bool WIDE> int run_dkv(const WinArgs& a, int B, int
   auto kern = k_win_dkv<T, D, WIDE>;
   constexpr size_t smem = Shape<T, D, WIDE>::kvb;
   static_assert(smem <= 160 * 1024, "LDS of a CU");
-  if (raise_lds((const void*)kern, smem, "window_attention_bwd")) return 1;
+  static std::atomic<uint64_t> done{0};
+  if (raise_lds((const void*)kern, smem, "window_attention_bwd", done)) return 1;
   hipLaunchKernelGGL(kern, dim3((a.sink_tiles * (a.nchunk - 1) + ktiles) * B * a.kv), dim3(256), smem, st, a);
   DP_CHECK_LAUNCH("window_attention_bwd(dkv)");
   if (a.sink_tiles) {
