@@ -188,7 +188,7 @@ template <typename T, int D> struct Frags {
 // matrix instruction in the forward kernel).  One where two would spill.
 template <typename T, int D, bool WIDE> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : sizeof(T) == 2 && D == 128 && WIDE ? 3 : 2; }
 template <typename T, int D> constexpr int waves_dq() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
-template <typename T, int D> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : 2; }
+template <typename T, int D, bool WIDE> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : sizeof(T) == 2 && D == 64 && WIDE ? 3 : 2; }
 
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
@@ -665,7 +665,7 @@ __device__ __forceinline__ Span tokens_of(const WinArgs& a, const Seq& s, int jl
 }
 
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -702,15 +702,15 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   for (int dt = 0; dt < C::DT; dt++) { ak[dt] = zero16(); av[dt] = zero16(); }
   const Span mine = live ? tokens_of(a, sq, j, j) : Span{0x7fffffff, 0x7fffffff};
   const Span block = k0 < sq.len ? tokens_of(a, sq, k0, min(k0 + S::ROWS, sq.len) - 1) : Span{0, 0};
-  // (tokens that all keys of the wave are seen by need no mask, tokens that see none of them no work)
-  int all_lo = mine.lo, all_hi = live ? mine.hi : 0, any_lo = mine.lo, any_hi = live ? mine.hi : 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all_lo = max(all_lo, __shfl_xor(all_lo, o, 64)); all_hi = min(all_hi, __shfl_xor(all_hi, o, 64));
-    any_lo = min(any_lo, __shfl_xor(any_lo, o, 64)); any_hi = max(any_hi, __shfl_xor(any_hi, o, 64));
+  // Tokens that see all keys of the wave need no mask, tokens that see none of them no work.  The first token that sees a key moves with the
+  // key; the last does too, but for the sinks, which everyone behind sees.
+  const int j0 = k0 + (WIDE ? 32 * wv : 0), j1 = min(j0 + 31, sq.len - 1), jn = max(j0, a.sinks);
+  int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
+  if (j0 <= j1) {
+    const Span first = tokens_of(a, sq, j0, j0), last = tokens_of(a, sq, j1, j1);
+    any_lo = first.lo; any_hi = j0 < a.sinks ? first.hi : last.hi;
+    all_lo = last.lo; all_hi = j0 + 31 != j1 ? 0 : jn <= j1 ? tokens_of(a, sq, jn, jn).hi : first.hi;
   }
-  all_lo = __builtin_amdgcn_readfirstlane(all_lo); all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-  any_lo = __builtin_amdgcn_readfirstlane(any_lo); any_hi = __builtin_amdgcn_readfirstlane(any_hi);
   // tiles of RT tokens of one query head, the heads of the group one after the other
   const int per_head = (block.hi - block.lo + S::RT - 1) / S::RT, ntile = per_head * a.group;
   const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t0 = chunk * per, t1 = min(ntile, t0 + per);
@@ -719,9 +719,9 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
     if (i0 >= any_hi || i0 + 32 <= any_lo) return;
     v16f s = zero16(), dp = zero16();
     if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return F.rows(vals, 0, k); }, s, dp);
-    else two_products<T, D, read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
-    // (heads of 96 and 128: no registers to read the k-major operands ahead)
-    constexpr int AH = C::ES == 2 && D >= 96 ? 0 : C::DT;
+    else two_products<T, D, WIDE && D == 64 && sizeof(T) == 2 ? 2 : read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
+    // (the k-major operands are read ahead where that leaves the waves per SIMD as they are)
+    constexpr int AH = C::ES == 2 && (WIDE ? D >= 64 : D >= 96) ? 0 : C::DT;
     Frag8<T> gt[C::DT], qt[C::DT];
 #pragma unroll
     for (int dt = 0; dt < AH; dt++) { gt[dt] = F.cols(gs, 32 * u, dt); qt[dt] = F.cols(qs, 32 * u, dt); }
