@@ -65,6 +65,23 @@ __device__ __forceinline__ Frag8<float> pack8(const float* p, float) {
   for (int i = 0; i < 8; i++) f.v[i] = p[i];
   return f;
 }
+// sum of the 8 values of a fragment, added to l (two values an instruction; of the rounded values, the ones the second product takes)
+// (the word is copied first: a bit cast of a vector's element itself always took element 0)
+__device__ __forceinline__ float add8(const Frag8<bf16_t>& f, float l) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) { const unsigned w = f.u[i]; l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false); }
+  return l;
+}
+__device__ __forceinline__ float add8(const Frag8<f16_t>& f, float l) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) { const unsigned w = f.u[i]; l = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false); }
+  return l;
+}
+__device__ __forceinline__ float add8(const Frag8<float>& f, float l) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) l += f.v[i];
+  return l;
+}
 template <typename T> __device__ __forceinline__ float elem(const Frag8<T>& f, int i) {
   const unsigned short h = (unsigned short)(f.u[i >> 1] >> (16 * (i & 1)));
   return ld_f((const T*)&h);
@@ -138,29 +155,37 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 // this wave's LDS reads are done: their tile may be filled again
 __device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// operand fragments of a staged tile
+// Operand fragments of a staged tile.  Lane addresses are formed once (with the wave's own part of LDS, `base`); tile, row and step are
+// constants behind them: an exclusive-or below SW + 1, the rest added, so they end up in the read's offset field.
 template <typename T, int D> struct Frags {
   using C = Cfg<T, D>;
   int row, fx, tr, tx;
-  __device__ __forceinline__ Frags(int lane) {
+  int ra[4], ca[2];      // 16-bit: the different lane addresses there are, kept in registers (formed anew for every step otherwise; heads of 128 have none to spare)
+  __device__ __forceinline__ Frags(int lane, int base) {
     const int c32 = lane & 31, h = lane >> 5, r = lane & 15, f = c32 & C::SW;
-    row = c32 * C::PITCH;
+    row = base + c32 * C::PITCH;
     fx = C::ES == 2 ? h ^ f : (2 * h) ^ f;
     if (C::ES == 2) {      // four rows of 16 channels per 16 lanes, transposed on the way
       const int tr_row = 4 * h + (r >> 2);
-      tr = tr_row * C::PITCH + 8 * (r & 1);
+      tr = base + tr_row * C::PITCH + 8 * (r & 1);
       tx = (2 * ((lane >> 4) & 1) + ((r >> 1) & 1)) ^ (tr_row & C::SW);
     } else {
-      tr = 4 * h * C::PITCH + 4 * (c32 & 3);
+      tr = base + 4 * h * C::PITCH + 4 * (c32 & 3);
       tx = (c32 >> 2) ^ (4 * h);
     }
+#pragma unroll
+    for (int i = 0; i < (C::SW + 1) / 2; i++) { ra[i] = row + (((2 * i) ^ fx) << 4); if (D < 128) asm("" : "+v"(ra[i])); }
+#pragma unroll
+    for (int i = 0; i < (C::SW + 1) / 4; i++) { ca[i] = tr + (((4 * i) ^ tx) << 4); if (D < 128) asm("" : "+v"(ca[i])); }
   }
+  // byte of piece p, swizzled by x
+  __device__ __forceinline__ static int piece(int p, int x) { return (((p & C::SW) ^ x) << 4) + ((p & ~C::SW) << 4); }
   // row (lane & 31) of the 32 rows from r0 on, channels 16 kk + 8 (lane >> 5) .. + 7
   __device__ __forceinline__ Frag8<T> rows(const char* tile, int r0, int kk) const {
-    const char* p = tile + r0 * C::PITCH + row;
-    if constexpr (C::ES == 2) { Frag8<T> f; f.u = *(const v4u*)(p + (((2 * kk) ^ fx) << 4)); return f; }
+    const char* p = tile + r0 * C::PITCH;
+    if constexpr (C::ES == 2) { Frag8<T> f; f.u = *(const v4u*)(p + ((2 * kk & ~C::SW) << 4) + ra[(2 * kk & C::SW) / 2]); return f; }
     else {
-      const v4f a = *(const v4f*)(p + (((4 * kk) ^ fx) << 4)), b = *(const v4f*)(p + (((4 * kk + 1) ^ fx) << 4));
+      const v4f a = *(const v4f*)(p + (row + piece(4 * kk, fx))), b = *(const v4f*)(p + (row + piece(4 * kk + 1, fx)));
       Frag8<T> f;
       f.v[0] = a[0]; f.v[1] = a[1]; f.v[2] = a[2]; f.v[3] = a[3]; f.v[4] = b[0]; f.v[5] = b[1]; f.v[6] = b[2]; f.v[7] = b[3];
       return f;
@@ -169,13 +194,13 @@ template <typename T, int D> struct Frags {
   // k-major: channel 32 dt + (lane & 31) of the 16 rows from r0 on, in the order of the accumulator registers (rows 4 h .. 4 h + 3 and
   // 8 + 4 h .. 8 + 4 h + 3 of lane half h)
   __device__ __forceinline__ Frag8<T> cols(const char* tile, int r0, int dt) const {
-    const char* p = tile + r0 * C::PITCH + tr;
-    if constexpr (C::ES == 2) return tr_pair<8 * D, T>((const T*)(p + (((4 * dt) ^ tx) << 4)));
+    const char* p = tile + r0 * C::PITCH;
+    if constexpr (C::ES == 2) return tr_pair<8 * D, T>((const T*)(p + ((4 * dt & ~C::SW) << 4) + ca[(4 * dt & C::SW) / 4]));
     else {
       Frag8<T> f;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const char* q = p + j * C::PITCH + 128 * dt + ((tx ^ j) << 4);
+        const char* q = p + j * C::PITCH + 128 * dt + (tr + ((tx ^ j) << 4));
         f.v[j] = *(const float*)q; f.v[4 + j] = *(const float*)(q + 8 * C::PITCH);
       }
       return f;
@@ -308,32 +333,38 @@ __device__ __forceinline__ void mask_keys(v16f& s, const Row& row, int k0, int h
 }
 
 // The stream of a block's tiles: tile(t, i) issues the copies of tile t into buffer i, land(i) stores what came in registers, work(t, i)
-// computes.  Two buffers: the copies of the next tile run while this one is worked on.  Wide: a wave passes the barrier when its own copies
-// have landed, so behind it everyone's have, and everyone is done with the buffer that is filled next.  Narrow: a wave by itself, every
-// fourth tile.
+// computes; i is a constant of the code (the loop holds both buffers' turns).  Two buffers: the copies of the next tile run while this one is
+// worked on.  Wide: a wave passes the barrier when its own copies have landed, so behind it everyone's have, and everyone is done with the
+// buffer that is filled next.  Narrow: a wave by itself, every fourth tile.
+template <int I> struct Buf { static constexpr int v = I; };
 template <typename S, typename TILE, typename LAND, typename WORK>
 __device__ __forceinline__ void stream_tiles(int t0, int t1, TILE tile, LAND land, WORK work) {
   constexpr int step = S::NTH == 256 ? 1 : 4;
-  if (S::NBUF == 2) {
-    int buf = 0;
-    if (t0 < t1) tile(t0, 0);
-    PROLOGUE_LOADED;
-    for (int t = t0; t < t1; t += step) {
+  int t = t0;
+  if constexpr (S::NBUF == 2) {
+    auto turn = [&](auto i) {
       loads_done();
-      land(buf);
+      land(i);
       if (S::NTH == 256) lds_barrier(); else reads_done();
-      if (t + step < t1) tile(t + step, buf ^ 1);
-      work(t, buf);
-      buf ^= 1;
+      if (t + step < t1) tile(t + step, Buf<1 - decltype(i)::v>());
+      work(t, i);
+      t += step;
+    };
+    if (t < t1) tile(t, Buf<0>());
+    PROLOGUE_LOADED;
+    while (t < t1) {
+      turn(Buf<0>());
+      if (t >= t1) break;
+      turn(Buf<1>());
     }
-    return;
-  }
-  for (int t = t0; t < t1; t += step) {
-    reads_done();
-    tile(t, 0);
-    loads_done();
-    land(0);
-    work(t, 0);
+  } else {
+    for (; t < t1; t += step) {
+      reads_done();
+      tile(t, Buf<0>());
+      loads_done();
+      land(Buf<0>());
+      work(t, Buf<0>());
+    }
   }
 }
 
@@ -367,7 +398,8 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
   float m = -INFINITY, mc = 0.f, l = 0.f;
   const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
   const int per = (pl.nt + a.nsplit - 1) / a.nsplit, t0 = split * per, t1 = min(pl.nt, t0 + per);
-  const Frags<T, D> F(lane);
+  const int own = WIDE ? 0 : wv * S::NBUF * 2 * S::tile;      // the wave's tiles
+  const Frags<T, D> F(lane, own);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
   auto step = [&](const char* ks, const char* vs, int u, int k0) {      // 32 keys, k0 the first of them, rows 32 u .. of the tile
@@ -406,8 +438,9 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
     for (int st = 0; st < 2; st++) {
       float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -mc)); l += p[i]; }
+      for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * st + i], a.c, -mc));
       const Frag8<T> pf = pack8(p, T{});
+      l = add8(pf, l);
       Frag8<T> vn[C::DT];
       if (st == 0) {
 #pragma unroll
@@ -421,17 +454,16 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
 
   const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
   const Copy<T, D, S::KT, S::NTH, S::DIRECT> ck(a.k.t, gid), cv(a.v.t, gid);
-  char* const tiles = smem + (WIDE ? 0 : wv * S::NBUF * 2 * S::tile);
   stream_tiles<S>(WIDE ? t0 : t0 + wv, t1,
-    [&](int t, int i) {
+    [&](int t, auto i) {
       const int k0 = key_of(t);
-      char* at = tiles + i * 2 * S::tile;
+      char* at = smem + own + decltype(i)::v * 2 * S::tile;
       ck.issue(Kb, a.k.t, k0, sq.len - k0, at, wave_id); cv.issue(Vb, a.v.t, k0, sq.len - k0, at + S::tile, wave_id);
     },
-    [](int) {},
-    [&](int t, int i) {
+    [](auto) {},
+    [&](int t, auto i) {
       const int k0 = key_of(t);
-      const char* at = tiles + i * 2 * S::tile;
+      const char* at = smem + decltype(i)::v * 2 * S::tile;
 #pragma unroll
       for (int u = 0; u < S::KS; u++) step(at, at + S::tile, u, k0 + 32 * u);
     });
@@ -564,7 +596,8 @@ __global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArg
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
   const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
-  const Frags<T, D> F(lane);
+  const int own = WIDE ? 0 : wv * S::NBUF * 2 * S::tile;      // the wave's tiles
+  const Frags<T, D> F(lane, own);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
   auto step = [&](const char* ks, const char* vs, int u, int k0) {
@@ -597,17 +630,16 @@ __global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArg
 
   const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
   const Copy<T, D, S::KT, S::NTH, S::DIRECT> ck(a.k.t, gid), cv(a.v.t, gid);
-  char* const tiles = smem + (WIDE ? 0 : wv * S::NBUF * 2 * S::tile);
   stream_tiles<S>(WIDE ? 0 : wv, pl.nt,
-    [&](int t, int i) {
+    [&](int t, auto i) {
       const int k0 = key_of(t);
-      char* at = tiles + i * 2 * S::tile;
+      char* at = smem + own + decltype(i)::v * 2 * S::tile;
       ck.issue(Kb, a.k.t, k0, sq.len - k0, at, wave_id); cv.issue(Vb, a.v.t, k0, sq.len - k0, at + S::tile, wave_id);
     },
-    [](int) {},
-    [&](int t, int i) {
+    [](auto) {},
+    [&](int t, auto i) {
       const int k0 = key_of(t);
-      const char* at = tiles + i * 2 * S::tile;
+      const char* at = smem + decltype(i)::v * 2 * S::tile;
 #pragma unroll
       for (int u = 0; u < S::KS; u++) step(at, at + S::tile, u, k0 + 32 * u);
     });
@@ -682,8 +714,8 @@ __global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const
   const T* Qb = (const T*)a.q.p + (int64_t)b * a.q.b + (int64_t)kvh * a.group * a.q.h;
   const T* Gb = (const T*)a.go.p + (int64_t)b * a.go.b + (int64_t)kvh * a.group * a.go.h;
   const float *lseb = a.lse + (int64_t)bh * a.rows, *dlb = a.delta + (int64_t)bh * a.rows;
-  const Frags<T, D> F(lane);
-  char* const vals = smem + S::vals + (WIDE ? wv * 32 * C::PITCH : 0);
+  const int set0 = WIDE ? 0 : wv * S::NBUF, own = set0 * 2 * S::rtile;      // the wave's tiles
+  const Frags<T, D> F(lane, own), FV(lane, WIDE ? wv * 32 * C::PITCH : 0);
   Frag8<T> kf[C::KK], vf[S::VLDS ? 1 : C::KK];
   {
     const int jc = live ? j : 0;       // (a key behind the sequence: any key, its column is thrown away)
@@ -693,7 +725,7 @@ __global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const
     for (int kk = 0; kk < C::KK; kk++) {
       kf[kk] = ldg8(Kr + 16 * kk + 8 * h);
       // (narrow: the four waves own the same keys and write the same values; a wave reads behind its own writes)
-      if constexpr (S::VLDS) *(v4u*)(vals + F.row + (((2 * kk) ^ F.fx) << 4)) = ldg8(Vr + 16 * kk + 8 * h).u;
+      if constexpr (S::VLDS) *(v4u*)(smem + S::vals + FV.row + FV.piece(2 * kk, FV.fx)) = ldg8(Vr + 16 * kk + 8 * h).u;
       else vf[kk] = ldg8(Vr + 16 * kk + 8 * h);
     }
   }
@@ -718,7 +750,7 @@ __global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const
   auto step = [&](const char* qs, const char* gs, const float* sl, const float* sd, int u, int i0) {      // 32 query rows, i0 the first token
     if (i0 >= any_hi || i0 + 32 <= any_lo) return;
     v16f s = zero16(), dp = zero16();
-    if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return F.rows(vals, 0, k); }, s, dp);
+    if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return FV.rows(smem + S::vals, 0, k); }, s, dp);
     else two_products<T, D, WIDE && D == 64 && sizeof(T) == 2 ? 2 : read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
     // (the k-major operands are read ahead where that leaves the waves per SIMD as they are)
     constexpr int AH = C::ES == 2 && (WIDE ? D >= 64 : D >= 96) ? 0 : C::DT;
@@ -767,24 +799,23 @@ __global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const
 
   const int gid = WIDE ? tid : lane, wave_id = WIDE ? wv : 0;
   const Copy<T, D, S::RT, S::NTH, S::DIRECT> cq(a.q.t, gid), cg(a.go.t, gid);
-  const int set0 = WIDE ? 0 : wv * S::NBUF;
   float ls = 0.f, dl = 0.f;
   auto stats_of = [&](int i) { return (float*)(smem + S::rstage + (set0 + i) * 512); };
   stream_tiles<S>(WIDE ? t0 : t0 + wv, t1,
-    [&](int t, int i) {
+    [&](int t, auto i) {
       // rows behind the block's tokens arrive as zeros, with zeros for lse and delta: P = 1 times a zero row of dO, dS = 0
       const int g = a.group == 1 ? 0 : t / per_head, i0 = block.lo + (t - g * per_head) * S::RT, left = block.hi - i0;
-      char* at = smem + (set0 + i) * 2 * S::rtile;
+      char* at = smem + own + decltype(i)::v * 2 * S::rtile;
       cq.issue(Qb + (int64_t)g * a.q.h, a.q.t, i0, left, at, wave_id); cg.issue(Gb + (int64_t)g * a.go.h, a.go.t, i0, left, at + S::rtile, wave_id);
       const bool in = gid < min(left, S::RT);
       const int64_t r = (int64_t)(i0 + (in ? gid : 0)) * a.group + g;
       ls = in ? lseb[r] : 0.f; dl = in ? dlb[r] : 0.f;
     },
-    [&](int i) { if (gid < S::RT) { float* st = stats_of(i); st[gid] = ls; st[64 + gid] = dl; } },
-    [&](int t, int i) {
+    [&](auto i) { if (gid < S::RT) { float* st = stats_of(decltype(i)::v); st[gid] = ls; st[64 + gid] = dl; } },
+    [&](int t, auto i) {
       const int i0 = block.lo + (a.group == 1 ? t : t % per_head) * S::RT;
-      const char* at = smem + (set0 + i) * 2 * S::rtile;
-      const float* st = stats_of(i);
+      const char* at = smem + decltype(i)::v * 2 * S::rtile;
+      const float* st = stats_of(decltype(i)::v);
 #pragma unroll
       for (int u = 0; u < S::RS; u++) step(at, at + S::rtile, st, st + 64, u, i0 + 32 * u);
     });
