@@ -392,14 +392,43 @@ class PatchEmbeddingBlock(nn.Module):
 
 
 class SABlock(nn.Module):
-    def __init__(self, hidden_size, num_heads, dropout_rate=0.0):
+    """Self-attention block.  The keyword arguments change what a token attends to and where it stands (ops.window_attention_qkv); without them
+    the block is the reference's, and so are its keys:
+    window: None (all tokens), n or (left, right): a token sees that many before and behind it, None for no limit on a side;
+    sinks: the first tokens stay visible to every token; qk_norm: LayerNorm of every head's queries and keys (keys q_norm.*, k_norm.*);
+    rotary: rotated pairs of a head per axis of the positions that forward() is given; base, interleaved: as in ops.rotary_axes."""
+
+    def __init__(self, hidden_size, num_heads, dropout_rate=0.0, *, window=None, sinks=0, qk_norm=False, rotary=None, base=10000.0,
+                 interleaved=False):
         super().__init__()
         self.num_heads = num_heads
         self.out_proj = nn.Linear(hidden_size, hidden_size)
         self.qkv = nn.Linear(hidden_size, hidden_size * 3, bias=False)
+        self.left, self.right = window if isinstance(window, (tuple, list)) else (window, window)
+        self.sinks, self.qk_norm, self.base, self.interleaved = sinks, bool(qk_norm), base, interleaved
+        self.rotary = tuple(rotary) if rotary is not None else None
+        if sinks and self.left is None:
+            raise ValueError("sinks need a limit on the left of the window")
+        self.full = self.left is None and self.right is None and not qk_norm and rotary is None
+        if not self.full:
+            ops.check_attention_options(hidden_size, num_heads, self.left, self.right, sinks, self.rotary, base, interleaved)
+        if qk_norm:
+            self.q_norm = nn.LayerNorm(hidden_size // num_heads)
+            self.k_norm = nn.LayerNorm(hidden_size // num_heads)
 
-    def forward(self, x):
-        o = ops.attention(ops.linear(x, self.qkv.weight, defer_wgrad=True), self.num_heads)
+    def forward(self, x, positions=None):
+        if self.rotary is not None and positions is None:
+            raise ValueError("SABlock: a block with rotary needs the tokens' positions")
+        qkv = ops.linear(x, self.qkv.weight, defer_wgrad=True)
+        if self.full:
+            o = ops.attention(qkv, self.num_heads)
+        else:
+            norm, eps = None, 1e-5
+            if self.qk_norm:
+                norm, eps = (self.q_norm.weight, self.q_norm.bias, self.k_norm.weight, self.k_norm.bias), self.q_norm.eps
+            o = ops.window_attention_qkv(qkv, self.num_heads, left=self.left, right=self.right, sinks=self.sinks, norm=norm, eps=eps,
+                                         positions=positions if self.rotary is not None else None, sections=self.rotary, base=self.base,
+                                         interleaved=self.interleaved)
         return ops.linear(o, self.out_proj.weight, self.out_proj.bias, defer_wgrad=True)
 
 
@@ -415,23 +444,27 @@ class MLPBlock(nn.Module):
 
 
 class TransformerBlock(nn.Module):
-    def __init__(self, hidden_size, mlp_dim, num_heads, dropout_rate=0.0):
+    """attention: keyword arguments of SABlock."""
+
+    def __init__(self, hidden_size, mlp_dim, num_heads, dropout_rate=0.0, attention=None):
         super().__init__()
         self.mlp = MLPBlock(hidden_size, mlp_dim, dropout_rate)
         self.norm1 = nn.LayerNorm(hidden_size)
-        self.attn = SABlock(hidden_size, num_heads, dropout_rate)
+        self.attn = SABlock(hidden_size, num_heads, dropout_rate, **(attention or {}))
         self.norm2 = nn.LayerNorm(hidden_size)
 
-    def forward(self, x):
-        x = ops.add(x, self.attn(ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)))
+    def forward(self, x, positions=None):
+        x = ops.add(x, self.attn(ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps), positions))
         return ops.add(x, self.mlp(ops.layer_norm(x, self.norm2.weight, self.norm2.bias, self.norm2.eps)))
 
 
 class ViT(nn.Module):
-    """MONAI 0.7.0 ViT(classification=False): returns (LayerNorm(last), [every block's output])."""
+    """MONAI 0.7.0 ViT(classification=False): returns (LayerNorm(last), [every block's output]).
+    attention: None (the reference's blocks) or keyword arguments of SABlock for every block; rotary=True there divides a head's pairs evenly
+    over the axes of the patch grid, whose coordinates are the positions."""
 
     def __init__(self, in_channels, img_size, patch_size, hidden_size=768, mlp_dim=3072, num_layers=12, num_heads=12,
-                 pos_embed="conv", classification=False, num_classes=2, dropout_rate=0.0, spatial_dims=3):
+                 pos_embed="conv", classification=False, num_classes=2, dropout_rate=0.0, spatial_dims=3, attention=None):
         super().__init__()
         if not (0 <= dropout_rate <= 1):
             raise ValueError("dropout_rate should be between 0 and 1.")
@@ -441,7 +474,20 @@ class ViT(nn.Module):
             raise ValueError("HIP path implements dropout_rate=0 (the reference's setting)")
         self.patch_embedding = PatchEmbeddingBlock(in_channels, img_size, patch_size, hidden_size, num_heads, pos_embed,
                                                    dropout_rate, spatial_dims)
-        self.blocks = nn.ModuleList([TransformerBlock(hidden_size, mlp_dim, num_heads, dropout_rate) for _ in range(num_layers)])
+        attention = dict(attention or {})
+        rotary = attention.get("rotary")
+        if rotary is True:
+            attention["rotary"] = (hidden_size // num_heads // (2 * len(patch_size)),) * len(patch_size)
+        elif rotary is False:
+            attention["rotary"] = None
+        elif rotary is not None and len(tuple(rotary)) != len(patch_size):
+            raise ValueError(f"rotary {rotary}: one number of pairs per axis of the {len(patch_size)}-dimensional patch grid")
+        positions = None
+        if attention.get("rotary") is not None:      # the patches' order: the last axis runs fastest
+            axes = [torch.arange(i // p, dtype=torch.int32) for i, p in zip(img_size, patch_size)]
+            positions = torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, len(axes))
+        self.register_buffer("positions", positions, persistent=False)
+        self.blocks = nn.ModuleList([TransformerBlock(hidden_size, mlp_dim, num_heads, dropout_rate, attention) for _ in range(num_layers)])
         self.norm = nn.LayerNorm(hidden_size)
         for m in self.blocks.modules():
             if isinstance(m, nn.Linear):
@@ -461,7 +507,7 @@ class ViT(nn.Module):
         first = self.blocks[0]
         n = ops.layer_norm(x, first.norm1.weight, first.norm1.bias, first.norm1.eps)
         for i, blk in enumerate(self.blocks):
-            x, n = ops.add_layer_norm(x, blk.attn(n), blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
+            x, n = ops.add_layer_norm(x, blk.attn(n, self.positions), blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
             nxt = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
             x, n = ops.add_layer_norm(x, blk.mlp(n), nxt.weight, nxt.bias, nxt.eps)
             hidden.append(x)

@@ -1,6 +1,6 @@
 """DOSE-PYFER on the HIP path.  Mirrors DosePrediction/Models/Networks/dose_pyfer.py: class names, constructor
 signatures, ValueErrors, state_dict keys and forward I/O ([output_A, [out128, out64, out32, out16]], NCDHW fp32)."""
-from typing import Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -132,12 +132,12 @@ class small_blocks_beside:
 
 
 class ViTEncoder(nn.Module):
-    """dose_pyfer.ViTEncoder (22-144)."""
+    """dose_pyfer.ViTEncoder (22-144).  attention: options of the transformer's attention (blocks.ViT); None: the reference's."""
 
     def __init__(self, in_channels: int, img_size: Union[Sequence[int], int], feature_size: int = 16, hidden_size: int = 768,
                  mlp_dim: int = 3072, num_heads: int = 12, num_layers: int = 12, pos_embed: str = "conv",
                  norm_name: Union[Tuple, str] = "instance", conv_block: bool = True, res_block: bool = True,
-                 dropout_rate: float = 0.0, spatial_dims: int = 3) -> None:
+                 dropout_rate: float = 0.0, spatial_dims: int = 3, attention: Optional[dict] = None) -> None:
         super().__init__()
         if not (0 <= dropout_rate <= 1):
             raise ValueError("dropout_rate should be between 0 and 1.")
@@ -151,7 +151,7 @@ class ViTEncoder(nn.Module):
         self.classification = False
         self.vit = ViT(in_channels=in_channels, img_size=img_size, patch_size=self.patch_size, hidden_size=hidden_size,
                        mlp_dim=mlp_dim, num_layers=self.num_layers, num_heads=num_heads, pos_embed=pos_embed,
-                       classification=self.classification, dropout_rate=dropout_rate, spatial_dims=spatial_dims)
+                       classification=self.classification, dropout_rate=dropout_rate, spatial_dims=spatial_dims, attention=attention)
         self.skip1 = UnetrBasicBlock(spatial_dims, in_channels, feature_size, kernel_size=3, stride=1, norm_name=norm_name,
                                      res_block=res_block)
         self.skip2 = UnetrPrUpBlock(spatial_dims, hidden_size, feature_size * 2, num_layer=2, kernel_size=3, stride=1,
@@ -227,11 +227,12 @@ class MainSubsetModel(nn.Module):
 
     def __init__(self, in_ch, out_ch, img_size, feature_size: int = 16, hidden_size: int = 768, mlp_dim: int = 3072,
                  num_heads: int = 12, num_layers: int = 12, conv_block: bool = True, res_block: bool = True,
-                 dropout_rate: float = 0.0, mode_multi_dec=False, act="relu", multiS_conv=True):
+                 dropout_rate: float = 0.0, mode_multi_dec=False, act="relu", multiS_conv=True, attention=None):
         super().__init__()
         self.encoder = ViTEncoder(in_channels=in_ch, img_size=img_size, feature_size=feature_size, hidden_size=hidden_size,
                                   mlp_dim=mlp_dim, num_heads=num_heads, num_layers=num_layers, pos_embed="perceptron",
-                                  norm_name="instance", res_block=res_block, conv_block=conv_block, dropout_rate=dropout_rate)
+                                  norm_name="instance", res_block=res_block, conv_block=conv_block, dropout_rate=dropout_rate,
+                                  attention=attention)
         self.decoder = PyMSCDecoder(feature_size=feature_size, hidden_size=hidden_size, mode_multi=mode_multi_dec, act=act,
                                     multiS_conv=multiS_conv)
 
@@ -259,12 +260,12 @@ class Model(nn.Module):
     """dose_pyfer.Model (325-360): net_A (C3D U-Net) -> cat(out_A, x) -> net_B; returns [output_A, out_net_B]."""
 
     def __init__(self, in_ch, out_ch, list_ch_A, feature_size=16, img_size=(128, 128, 128), num_layers=8, num_heads=6,
-                 act="mish", mode_multi_dec=True, multiS_conv=True):
+                 act="mish", mode_multi_dec=True, multiS_conv=True, attention=None):
         super().__init__()
         self.net_A = BaseUNet(in_ch, list_ch_A)
         self.net_B = MainSubsetModel(in_ch=in_ch + list_ch_A[1], out_ch=out_ch, feature_size=feature_size, img_size=img_size,
                                      num_layers=num_layers, num_heads=num_heads, act=act, mode_multi_dec=mode_multi_dec,
-                                     multiS_conv=multiS_conv)
+                                     multiS_conv=multiS_conv, attention=attention)
         self.conv_out_A = nn.Conv3d(list_ch_A[1], out_ch, kernel_size=1, padding=0, bias=True)
 
     def forward(self, x):
@@ -281,11 +282,11 @@ class Model(nn.Module):
 
 
 def create_pretrained_unet(ckpt_file, in_ch, out_ch, list_ch_A, feature_size, img_size, num_layers=8, num_heads=6, act="mish",
-                           mode_multi_dec=True, multiS_conv=True):
+                           mode_multi_dec=True, multiS_conv=True, attention=None):
     """dose_pyfer.create_pretrained_unet (363-407): load by key intersection, strict=False."""
     pretrain = torch.load(ckpt_file, map_location="cpu")
     net = Model(in_ch, out_ch, list_ch_A, feature_size=feature_size, img_size=img_size, num_layers=num_layers,
-                num_heads=num_heads, act=act, mode_multi_dec=mode_multi_dec, multiS_conv=multiS_conv)
+                num_heads=num_heads, act=act, mode_multi_dec=mode_multi_dec, multiS_conv=multiS_conv, attention=attention)
     net_dict = net.state_dict()
     inside = tuple({k for k in pretrain["network_state_dict"] if k in net_dict.keys()})
     pretrain["network_state_dict"] = {k: v for k, v in pretrain["network_state_dict"].items() if k in net_dict.keys()}

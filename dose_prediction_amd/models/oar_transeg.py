@@ -1,6 +1,6 @@
 """OAR-TRANSEG on the HIP path.  Mirrors OARSegmentation/Models/Networks/oar_transeg.py:14-185 (and, with ``old=True`` /
 class TRANSEG, the OldModels variant the shipped trainer imports)."""
-from typing import Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch.nn as nn
 
@@ -11,12 +11,13 @@ from .dose_pyfer import ensure_tuple_rep, run_vit_beside, small_blocks_beside
 
 
 class Model(nn.Module):
+    """attention: options of the transformer's attention (blocks.ViT); None: the reference's."""
     _OLD = False
 
     def __init__(self, in_channels: int, out_channels: int, img_size: Union[Sequence[int], int], feature_size: int = 16,
                  hidden_size: int = 768, mlp_dim: int = 3072, num_heads: int = 12, pos_embed: str = "conv",
                  norm_name: Union[Tuple, str] = "instance", conv_block: bool = True, res_block: bool = True,
-                 dropout_rate: float = 0.0, spatial_dims: int = 3) -> None:
+                 dropout_rate: float = 0.0, spatial_dims: int = 3, attention: Optional[dict] = None) -> None:
         super().__init__()
         if not (0 <= dropout_rate <= 1):
             raise ValueError("dropout_rate should be between 0 and 1.")
@@ -30,7 +31,7 @@ class Model(nn.Module):
         self.classification = False
         self.vit = ViT(in_channels=in_channels, img_size=img_size, patch_size=self.patch_size, hidden_size=hidden_size,
                        mlp_dim=mlp_dim, num_layers=self.num_layers, num_heads=num_heads, pos_embed=pos_embed,
-                       classification=self.classification, dropout_rate=dropout_rate, spatial_dims=spatial_dims)
+                       classification=self.classification, dropout_rate=dropout_rate, spatial_dims=spatial_dims, attention=attention)
         self.encoder1 = UnetrBasicBlock(spatial_dims, in_channels, feature_size, kernel_size=3, stride=1, norm_name=norm_name,
                                         res_block=res_block)
         self.encoder2 = UnetrPrUpBlock(spatial_dims, hidden_size, feature_size * 2, num_layer=2, kernel_size=3, stride=1,

@@ -2607,6 +2607,15 @@ def window_attention(q, k, v, left=None, right=None, sinks=0, q_start=0, lengths
     return WindowAttention.apply(q, k, v, win, int(q_start), starts, lengths)
 
 
+def check_attention_options(width, heads, left, right, sinks, sections, base, interleaved):
+    """What window_attention_qkv checks of a configuration, for a module to check when it is built."""
+    what = "window_attention_qkv"
+    d = _head_dim(width, heads, what)
+    _window_args(what, left, right, sinks, None, d)
+    if sections is not None:
+        _rotary_plan(what, d, tuple(sections), base, interleaved)
+
+
 class WindowAttentionQkv(torch.autograd.Function):
     """The packed projection's form: norm and rotation of q and k into a buffer of their own (one launch, none without them), v read in
     place; the backward pass writes one packed gradient, that of q and k passing through the norm and the rotation unrounded (float)."""
