@@ -221,8 +221,9 @@ struct WinArgs {
   float *lse, *delta, *part;      // delta: rowsum(dO O) * scale
   const int *starts, *lens;
   int kv, group, Nq, Nk, rows, left, right, sinks, start, tiles, nsplit, sink_tiles, nchunk, g_f32;
-  float c, scale;
+  float c, lag, scale;      // c = scale * log2(e); lag: LAG powers of two in units of a score
 };
+constexpr float LAG = 8.f;
 
 // contiguous ranges of the (batch, key head, tile) space per XCD: the blocks of one XCD's L2 read the same keys
 __device__ __forceinline__ int xcd_range(int id, int total) {
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
   v16f acc[C::DT];
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++) acc[dt] = zero16();
-  float m = -INFINITY, mc = 0.f, l = 0.f;
+  float lim = -INFINITY, mc = 0.f, l = 0.f;      // nothing seen yet: lim = -inf, mc = 0
   const Plan pl = key_tiles<S::KT>(a, sq.len, sq.start + r0 / a.group, sq.start + (min(r0 + S::ROWS, a.rows) - 1) / a.group);
   const int per = (pl.nt + a.nsplit - 1) / a.nsplit, t0 = split * per, t1 = min(pl.nt, t0 + per);
   const int own = WIDE ? 0 : wv * S::NBUF * 2 * S::tile;      // the wave's tiles
@@ -426,11 +427,13 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-    const float mn = fmaxf(m, pair_max(mx));
-    if (__builtin_amdgcn_ballot_w64(mn > m)) {        // (the maximum of a row moves in its first tiles, hardly ever after them)
-      // (alpha from the rounded products: exactly 1 for the rows whose maximum stays, whatever the wave's other rows hold)
-      const float nc = mn == -INFINITY ? 0.f : mn * a.c, alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - nc);
-      m = mn; mc = nc; l *= alpha;
+    // The subtracted maximum lags behind: it moves when a score passes it by more than LAG (in powers of two), so that P <= 2^LAG -- the
+    // relative precision of P, its sum and the products is the same -- and the first tiles do not rescale the accumulators one after another.
+    // (Every row decides for itself: one that stays has alpha = 2^0, exactly 1, whatever the wave's other rows do.)
+    mx = pair_max(mx);
+    if (__builtin_amdgcn_ballot_w64(mx > lim)) {
+      const float nc = mx > lim ? mx * a.c : mc, alpha = lim == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - nc);
+      lim = mx > lim ? mx + a.lag : lim; mc = nc; l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < C::DT; dt++) acc[dt] *= alpha;
     }
@@ -488,12 +491,12 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
     return;
   }
 
-  if (!row.live) { l = 0.f; m = -INFINITY; }
+  if (!row.live) { l = 0.f; lim = -INFINITY; }
   float* part = (float*)smem;
   float* mw = (float*)(smem + S::big);
   float* lw = mw + 4 * 32;
   __syncthreads();      // every wave is done with its tiles
-  if (h == 0) { mw[wv * 32 + c32] = m == -INFINITY ? -INFINITY : mc; lw[wv * 32 + c32] = l; }
+  if (h == 0) { mw[wv * 32 + c32] = lim == -INFINITY ? -INFINITY : mc; lw[wv * 32 + c32] = l; }
 #pragma unroll
   for (int dt = 0; dt < C::DT; dt++)
 #pragma unroll
@@ -1017,7 +1020,7 @@ extern "C" int dp_window_attention_fwd(const void* q, int64_t qb, int64_t qt, in
   a.kv = kv_heads; a.group = heads / kv_heads; a.Nq = Nq; a.Nk = Nk; a.rows = Nq * a.group;
   a.left = left < 0 ? FAR : left < FAR ? left : FAR; a.right = right < 0 ? FAR : right < FAR ? right : FAR; a.sinks = sinks < FAR ? sinks : FAR;
   a.start = q_start < -FAR ? -FAR : q_start > FAR ? FAR : q_start;
-  a.scale = scale; a.c = scale * LOG2E;
+  a.scale = scale; a.c = scale * LOG2E; a.lag = LAG / a.c;
   const Launch p = plan(B, kv_heads, a.group, Nq, Nk, d, a.left, a.right, a.sinks);
   a.tiles = p.tiles; a.nsplit = p.nsplit; a.nchunk = 1;
   if (p.nsplit > 1 && (!ws || ((uintptr_t)ws & 15))) DP_FAIL("window_attention_fwd: needs a 16-byte aligned workspace (dp_window_attention_ws_elems)");
