@@ -2518,6 +2518,8 @@ def _per_sequence(what, name, t, B, like):
         raise ValueError(f"{what}: {name} is int32 or int64 [{B}], got {t.dtype} {tuple(t.shape)}")
     if t.device != like.device:
         raise _lib.DoseHipError(f"{what}: {name} on {t.device}, rows on {like.device}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 30), 1 << 30)      # (a number past 32 bits stays past every row)
     return t.to(torch.int32).contiguous()
 
 

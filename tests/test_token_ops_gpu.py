@@ -257,6 +257,37 @@ def test_peaked_scores_and_scale(dtype):
             within(got, val, bound, what, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("step", [0.02, 0.4, 5.0])
+def test_rising_scores(dtype, step):
+    """Every key scores higher than the one before it, a window at a time: the running maximum creeps, steps and jumps, P passes 1 in between."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    B, N, heads, d = 2, 300, 2, 64
+    q = rnd((B, N, heads, d), 41, dev, scale=0.1)
+    q[..., 0] = 8.0
+    k = rnd((B, N, heads, d), 42, dev, scale=0.1)
+    k[..., 0] = (step * torch.arange(N, device=dev) - step * 150).view(1, N, 1)
+    q, k, v, g = (t.to(dtype) for t in (q, k, rnd((B, N, heads, d), 43, dev), rnd((B, N, heads, d), 44, dev)))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    for win in (dict(), dict(left=70, right=40, sinks=3), dict(right=0)):
+        out = ops.window_attention(*leaves, **win)
+        grads = torch.autograd.grad(out, leaves, g)
+        want = R.window(q.detach(), k.detach(), v.detach(), g, dtype=dtype, **win)
+        for what, got, (val, bound) in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), want):
+            within(got, val, bound, what, dtype)
+
+
+def test_lengths_and_starts_past_32_bits():
+    from dose_prediction_amd import ops
+    dev = _dev()
+    q, k, v = (rnd((3, 40, 2, 64), 45 + i, dev) for i in range(3))
+    big = torch.tensor([(1 << 32) + 3, 1 << 40, -(1 << 35)], device=dev)
+    got = ops.window_attention(q, k, v, left=9, lengths=big)
+    assert torch.equal(got, ops.window_attention(q, k, v, left=9, lengths=torch.tensor([40, 40, 0], device=dev)))
+    assert ops.window_attention(q, k, v, left=9, q_start=big).abs().max().item() == 0
+
+
 def test_gradient_against_differences():
     """Directional derivative of the fp32 kernels: central differences with h = 2^-6 are off by h^2 times the third derivative (scores change by
     at most ~0.3 here: below 2e-3 of the terms' size) and by 2 E |f| / h."""
