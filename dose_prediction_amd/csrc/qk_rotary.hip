@@ -9,9 +9,12 @@
 // Bound: HBM.  A value is read once and written once (the backward pass reads x and gy, writes gx; the row statistics are recomputed from
 // the x that is in registers anyway, so nothing but x is kept between the passes).
 // Split: a lane owns 8 PAIRS of one head (16 channels, whole 16-byte pieces next to its neighbours'), so that a turn needs no other lane and a
-// head is d / 16 lanes whose sums are two or three shuffles.  Cosines and sines belong to a token, not to a head: a block computes those of its tokens once into LDS and all
-// heads of q and k share them.  Angles are formed in 64 bits (position * frequency, reduced to a fraction of a turn) because a far position
-// times a frequency has no fraction left in 32.
+// head is d / 16 lanes whose sums are two or three shuffles.  Cosines and sines belong to a token, not to a head: a block computes those of its
+// tokens once into LDS and all heads of q and k share them.  Angles are formed in 64 bits (position * frequency, reduced to a fraction of a
+// turn) because a far position times a frequency has no fraction left in 32.
+// Measured: turning 27 648 bf16 rows of 12 heads of 64 (85 MB in and out) 15.6 us; with the norm, 13 801 fp32 rows of 16 heads of 64: forward
+// 21.6 us (113 MB), backward 37 + 4 us for the weights' sums (170 MB); a large copy moves 4.9 TB/s, what a kernel before left in the cache comes
+// faster.
 #include "common.h"
 #include <math.h>
 
@@ -332,7 +335,8 @@ int check_rows(const char* name, const void* p, int64_t sb, int64_t st, int es) 
 }
 
 // tokens per block: enough of them that the angles (one per token and pair) spread over all threads, fewer where the grid would not
-// fill the 256 CUs
+// fill the 256 CUs.  (One token a block: 28 us instead of 15.6 at 27 648 tokens, with the norm 46 and 103 instead of 22 and 37 at 13 801; eight
+// at the 1024 tokens of two 128^3 volumes: 8.7 and 14.2 us instead of 7.2 and 12.6.)
 int block_tokens(int64_t tokens) { return tokens >= 8192 ? 8 : tokens >= 2048 ? 4 : tokens >= 512 ? 2 : 1; }
 
 }  // namespace

@@ -12,6 +12,13 @@
 // Matrix tiles are 32 x 32 (k = 16).  The score tile is computed transposed (streamed rows x owned columns): a lane then holds one owned
 // row's scores, and the accumulator registers are, pair by pair of 8-row groups, the B operand of the second product; its A operand is
 // the streamed tile read k-major from LDS (ds_read_b64_tr_b16).  Running maximum and sum are one register per lane, fp32.
+//
+// Roundings below 32 bits: P and dS go through the second product in the storage type (the matrix cores take nothing wider there), each off by
+// half a step of its own size; everything that is added up stays fp32.
+// Bound: the matrix cores and the exponentials beside them.  12 heads of 64, 13 825 tokens, window 577 + 576, one sink, bf16: forward 81 us,
+// dQ 102, dK / dV 136 + 5 for the sinks' sums; 6 heads of 128, window 1153 + 1152: 129, 209, 337 us.  Per 64 more keys a row the three take
+// 1.07, 1.27 and 1.27 PFLOP/s (measured over windows of 577 .. 2305 keys: what a large library product reaches is 1.22); the rest, a quarter at
+// that window, is the operands' first reading, which blocks that start together do not hide, and the tiles at the window's two edges.
 #include "common.h"
 #include <atomic>
 
@@ -428,7 +435,8 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
 #pragma unroll
     for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
     // The subtracted maximum lags behind: it moves when a score passes it by more than LAG (in powers of two), so that P <= 2^LAG -- the
-    // relative precision of P, its sum and the products is the same -- and the first tiles do not rescale the accumulators one after another.
+    // relative precision of P, its sum and the products is the same -- and the first tiles do not rescale the accumulators one after another
+    // (some row of 32 sees a new maximum in most of its first 40 tiles: 90 -> 81 us at the window of 1153 keys, heads of 64).
     // (Every row decides for itself: one that stays has alpha = 2^0, exactly 1, whatever the wave's other rows do.)
     mx = pair_max(mx);
     if (__builtin_amdgcn_ballot_w64(mx > lim)) {
@@ -905,6 +913,14 @@ int raise_lds(const void* kern, size_t smem, const char* name, std::atomic<uint6
 }
 
 // Which kernel, how many blocks: decided by sizes alone.
+// Wide where it gives every CU a block, narrow below (bf16, window 256 + 256, two sequences; forward / dQ / dK, dV in us, wide against narrow):
+//   heads of 128:  96 wide blocks 21 / 27 / 38 against 15 / 20 / 22;  264: 27 / 37 / 51 against 34 / 43 / 51
+//   heads of 64:  192: 15 / 18 / 22 against 16 / 20 / 22;  264: 16 / 19 / 23 against 20 / 25 / 27;  384: 20 / 25 / 29 against 26 / 32 / 36
+// Few rows, many keys (fewer than 256 narrow blocks): the key tiles are shared out over about 512 blocks, each with four tiles a wave or more
+// (a token of 12 heads on 4 key heads, 4 sequences of up to 32 769 keys, fp16: 22.1 + 4.3 us for the merge; over 256 blocks 22.9 + 4.0, over 1024
+// 23.6 + 6.3).
+// Tiles that hold sinks: their rows are dealt to as many blocks as have the work of another tile (dK / dV of 13 825 tokens, heads of 64: 143 us;
+// with one block a tile 519).
 struct Launch { bool wide; int tiles, nsplit; bool kwide; int ktiles, sink_tiles, nchunk; };
 Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right, int sinks) {
   Launch p;
