@@ -367,6 +367,7 @@ extern "C" int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, 
   if (make_plan("qk_rotary_fwd", R, pos, pos_kind, posb, naxes, sec, base, interleaved, d)) return 1;
   const int64_t tokens = (int64_t)B * N;
   if (tokens == 0 || heads + kv_heads == 0) return 0;
+  if (!x || !y) DP_FAIL("qk_rotary_fwd: x or y missing");
   const int tok = block_tokens(tokens);
   if ((tokens + tok - 1) / tok > 0x7fffffff || (int64_t)tok * (heads + kv_heads) > 0x3fffffff) DP_FAIL("qk_rotary_fwd: too many rows");
   QkArgs a{x, nullptr, y, xb, xt, 0, 0, yb, yt, wq, bq, wk, bk, nullptr, eps, inverse ? -1.f : 1.f, heads, kv_heads, tok, N, tokens};
@@ -397,6 +398,7 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
     if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 32)), dim3(1024), 0, STREAM, (const float*)part, dw, 0, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd"); }
     return 0;
   }
+  if (!g || !gx) DP_FAIL("qk_rotary_bwd: g or gx missing");
   const int tok = block_tokens(tokens);
   if ((tokens + tok - 1) / tok > 0x7fffffff || (int64_t)tok * (heads + kv_heads) > 0x3fffffff) DP_FAIL("qk_rotary_bwd: too many rows");
   QkArgs a{x, g, gx, xb, xt, gb, gt, gxb, gxt, wq, nullptr, wk, nullptr, part, eps, 1.f, heads, kv_heads, tok, N, tokens};

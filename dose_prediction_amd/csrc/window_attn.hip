@@ -1032,6 +1032,7 @@ extern "C" int dp_window_attention_fwd(const void* q, int64_t qb, int64_t qt, in
   if (check_mat("window_attention_fwd", "q", a.q, es, B > 0 ? Nq : 0, d) || check_mat("window_attention_fwd", "k", a.k, es, B > 0 ? Nk : 0, d) || check_mat("window_attention_fwd", "v", a.v, es, B > 0 ? Nk : 0, d) ||
       check_mat("window_attention_fwd", "o", a.o, es)) return 1;
   if (B == 0 || Nq == 0) return 0;
+  if (!q || !o || (Nk > 0 && (!k || !v))) DP_FAIL("window_attention_fwd: q, k, v or o missing");
   a.lse = lse; a.part = ws; a.starts = q_starts; a.lens = lengths;
   a.kv = kv_heads; a.group = heads / kv_heads; a.Nq = Nq; a.Nk = Nk; a.rows = Nq * a.group;
   a.left = left < 0 ? FAR : left < FAR ? left : FAR; a.right = right < 0 ? FAR : right < FAR ? right : FAR; a.sinks = sinks < FAR ? sinks : FAR;
@@ -1059,7 +1060,8 @@ extern "C" int dp_window_attention_bwd(const void* q, int64_t qb, int64_t qt, in
   if (check_mat(name, "q", a.q, es, B > 0 ? Nq : 0, d) || check_mat(name, "k", a.k, es, B > 0 ? Nk : 0, d) || check_mat(name, "v", a.v, es, B > 0 ? Nk : 0, d) || check_mat(name, "o", a.o, es) ||
       check_mat(name, "go", a.go, es, B > 0 ? Nq : 0, d) || check_mat(name, "dq", a.dq, gs) || check_mat(name, "dk", a.dk, gs) || check_mat(name, "dv", a.dv, es)) return 1;
   if (B == 0) return 0;
-  if (Nq > 0 && (!lse || !delta)) DP_FAIL("%s: lse / delta missing", name);
+  if (Nq > 0 && (!q || !o || !go || !lse || !delta || !dq)) DP_FAIL("%s: q, o, go, lse, delta or dq missing", name);
+  if (Nk > 0 && (!k || !v || !dk || !dv)) DP_FAIL("%s: k, v, dk or dv missing", name);
   a.lse = (float*)lse; a.delta = delta; a.part = ws; a.starts = q_starts; a.lens = lengths;
   a.kv = kv_heads; a.group = heads / kv_heads; a.Nq = Nq; a.Nk = Nk; a.rows = Nq * a.group;
   a.left = left < 0 ? FAR : left < FAR ? left : FAR; a.right = right < 0 ? FAR : right < FAR ? right : FAR; a.sinks = sinks < FAR ? sinks : FAR;

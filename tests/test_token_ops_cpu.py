@@ -67,6 +67,25 @@ def test_c_refusals_of_window_attention(bad):
         _lib.call(*_fwd(**bad))
 
 
+def test_c_missing_pointers():
+    from dose_prediction_amd import _lib
+    for n in "qkvo":
+        with pytest.raises(_lib.DoseHipError, match="missing"):
+            _lib.call(*_fwd(**{n: 0}))
+    mats = [(4096, 0, 64, 64)] * 5 + [(4096,), (4096,)] + [(4096, 0, 64, 64)] * 3
+    for i in range(10):
+        args = [m if j != i else (0, *m[1:]) for j, m in enumerate(mats)]
+        with pytest.raises(_lib.DoseHipError, match="missing"):
+            _lib.call("dp_window_attention_bwd", *(x for m in args for x in m), 0, 0, 1, 2, 1, 4, 4, 64, 1, 1, 0, 0, 0, 0, 0.125, 1, 0)
+    for x, y in ((0, 4096), (4096, 0)):
+        rot = (1, 4, 1, 1, 64)
+        with pytest.raises(_lib.DoseHipError, match="missing"):
+            _lib.call("dp_qk_rotary_fwd", x, 512, 128, y, 512, 128, *rot, 0, 0, 0, 0, 1e-5, 4096, 0, 0, 3, 12, 10, 10, 0, 10000.0, 0, 0, 1, 0)
+        with pytest.raises(_lib.DoseHipError, match="missing"):
+            _lib.call("dp_qk_rotary_bwd", 4096, 512, 128, x, 512, 128, 0, y, 512, 128, 0, 0, *rot, 0, 0, 1e-5, 4096, 0, 0, 3, 12, 10, 10, 0, 10000.0, 0,
+                      1, 0)
+
+
 def test_c_calls_without_work():
     from dose_prediction_amd import _lib
     assert _lib.call(*_fwd(B=0)) == 0 and _lib.call(*_fwd(Nq=0)) == 0
