@@ -220,7 +220,7 @@ template <typename T, int D> struct Frags {
 // matrix instruction in the forward kernel).  One where two would spill.
 template <typename T, int D, bool WIDE> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : sizeof(T) == 2 && D == 128 && WIDE ? 3 : 2; }
 template <typename T, int D> constexpr int waves_dq() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
-template <typename T, int D, bool WIDE> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : sizeof(T) == 2 && D == 64 && WIDE ? 3 : 2; }
+template <typename T, int D> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : sizeof(T) == 2 && D == 64 ? 3 : 2; }
 
 struct Mat { void* p; int64_t b, t, h; };      // element strides of sequence, token and head
 struct WinArgs {
@@ -252,8 +252,10 @@ template <typename T, int D, bool WIDE> struct Shape {
   // different tiles through LDS of their own and are merged at the end: four times the blocks, a quarter of the chain.
   // (heads of 128: 32-key tiles and 168 registers, so that three blocks stay on a CU instead of two: 172 -> 156 us at 6 heads, window 1152)
   static constexpr int KS = (WIDE && C::ES == 2 && D < 128) ? 2 : 1, KT = 32 * KS, ROWS = WIDE ? 128 : 32, NTH = WIDE ? 256 : 64;
-  // tiles in LDS per stream: the next one arrives while one is worked on (narrow: where two still leave room for two blocks on a CU)
-  static constexpr int NBUF = WIDE || (C::ES == 2 && D <= 64) ? 2 : 1;
+  // tiles in LDS per stream: wide, the next one arrives while one is worked on; narrow, one, and more blocks on a CU instead (2 x 1024 tokens, 12
+  // heads of 64, window 513: 16.3 -> 12.8, 19.7 -> 16.2 and, with dK / dV at three waves, 21.3 -> 17.2 us; chains of 1153 keys: 27 -> 23, 32 -> 33,
+  // 44 -> 45)
+  static constexpr int NBUF = WIDE ? 2 : 1;
   static constexpr int tile = KT * C::PITCH, sets = (WIDE ? 1 : 4) * NBUF, stage = sets * 2 * tile;
   static constexpr bool DIRECT = stage <= 64 * 1024;
   static constexpr int merge = WIDE ? 0 : 4 * 32 * C::CP * 4, big = stage > merge ? stage : merge;
@@ -341,22 +343,21 @@ __device__ __forceinline__ void mask_keys(v16f& s, const Row& row, int k0, int h
 }
 
 // The stream of a block's tiles: tile(t, i) issues the copies of tile t into buffer i, land(i) stores what came in registers, work(t, i)
-// computes; i is a constant of the code (the loop holds both buffers' turns).  Two buffers: the copies of the next tile run while this one is
-// worked on.  Wide: a wave passes the barrier when its own copies have landed, so behind it everyone's have, and everyone is done with the
-// buffer that is filled next.  Narrow: a wave by itself, every fourth tile.
+// computes; i is a constant of the code (the loop holds both buffers' turns).  Wide: the copies of the next tile run while this one is worked on; a
+// wave passes the barrier when its own copies have landed, so behind it everyone's have, and everyone is done with the buffer that is filled
+// next.  Narrow: a wave by itself, every fourth tile.
 template <int I> struct Buf { static constexpr int v = I; };
 template <typename S, typename TILE, typename LAND, typename WORK>
 __device__ __forceinline__ void stream_tiles(int t0, int t1, TILE tile, LAND land, WORK work) {
-  constexpr int step = S::NTH == 256 ? 1 : 4;
   int t = t0;
   if constexpr (S::NBUF == 2) {
     auto turn = [&](auto i) {
       loads_done();
       land(i);
-      if (S::NTH == 256) lds_barrier(); else reads_done();
-      if (t + step < t1) tile(t + step, Buf<1 - decltype(i)::v>());
+      lds_barrier();
+      if (t + 1 < t1) tile(t + 1, Buf<1 - decltype(i)::v>());
       work(t, i);
-      t += step;
+      t++;
     };
     if (t < t1) tile(t, Buf<0>());
     PROLOGUE_LOADED;
@@ -366,7 +367,7 @@ __device__ __forceinline__ void stream_tiles(int t0, int t1, TILE tile, LAND lan
       turn(Buf<1>());
     }
   } else {
-    for (; t < t1; t += step) {
+    for (; t < t1; t += 4) {
       reads_done();
       tile(t, Buf<0>());
       loads_done();
@@ -708,12 +709,12 @@ __device__ __forceinline__ Span tokens_of(const WinArgs& a, const Seq& s, int jl
 }
 
 template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const WinArgs a) {
+__global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinArgs a) {
   using C = Cfg<T, D>;
   using S = Shape<T, D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, h = lane >> 5;
-  // the tiles that hold sinks are seen by (nearly) every row: their rows are dealt to nchunk blocks, added up afterwards
+  // the rows of the first sink_tiles tiles are dealt to nchunk blocks each, added up afterwards
   const int ktiles = (a.Nk + S::ROWS - 1) / S::ROWS, per_bh = a.sink_tiles * a.nchunk + ktiles - a.sink_tiles;
   const int flat = xcd_range(blockIdx.x, gridDim.x), bh = flat / per_bh, e = flat % per_bh, b = bh / a.kv, kvh = bh % a.kv;
   const bool shared_rows = e < a.sink_tiles * a.nchunk && a.nchunk > 1;
@@ -762,9 +763,9 @@ __global__ __launch_bounds__(256, (waves_kv<T, D, WIDE>())) void k_win_dkv(const
     if (i0 >= any_hi || i0 + 32 <= any_lo) return;
     v16f s = zero16(), dp = zero16();
     if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return FV.rows(smem + S::vals, 0, k); }, s, dp);
-    else two_products<T, D, WIDE && D == 64 && sizeof(T) == 2 ? 2 : read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
+    else two_products<T, D, D == 64 && sizeof(T) == 2 ? 2 : read_group<T, D>()>(F, qs, gs, 32 * u, kf, [&](int k) { return vf[k]; }, s, dp);
     // (the k-major operands are read ahead where that leaves the waves per SIMD as they are)
-    constexpr int AH = C::ES == 2 && (WIDE ? D >= 64 : D >= 96) ? 0 : C::DT;
+    constexpr int AH = C::ES == 2 && D >= 64 ? 0 : C::DT;
     Frag8<T> gt[C::DT], qt[C::DT];
 #pragma unroll
     for (int dt = 0; dt < AH; dt++) { gt[dt] = F.cols(gs, 32 * u, dt); qt[dt] = F.cols(qs, 32 * u, dt); }
@@ -918,10 +919,13 @@ int raise_lds(const void* kern, size_t smem, const char* name, std::atomic<uint6
 //   heads of 64:  192: 15 / 18 / 22 against 16 / 20 / 22;  264: 16 / 19 / 23 against 20 / 25 / 27;  384: 20 / 25 / 29 against 26 / 32 / 36
 // Few rows, many keys (fewer than 256 narrow blocks): the key tiles are shared out over about 512 blocks, each with four tiles a wave or more
 // (a token of 12 heads on 4 key heads, 4 sequences of up to 32 769 keys, fp16: 22.1 + 4.3 us for the merge; over 256 blocks 22.9 + 4.0, over 1024
-// 23.6 + 6.3).
+// 23.6 + 6.3).  Where a wave's chain is short the merge costs more than it saves, the more so the more rows there are: 2048 rows over 1024 keys
+// 10.5 us, split 7.6 + 4.4; 4096 over 2048 16.4 against 10.6 + 6.7; 5000 over 2500 (heads of 128) 26.8 against 18.2 + 7.4.
+// Few key tiles: the rows that see one are dealt out in the same way (dK / dV of 1024 tokens, 12 heads of 64 on 4, every token before: 15.7 + 3.9
+// us; one block a tile 31.9; 8 heads of 96 on 2, 1000 tokens: 19.0 + 4.0 against 49.5).
 // Tiles that hold sinks: their rows are dealt to as many blocks as have the work of another tile (dK / dV of 13 825 tokens, heads of 64: 143 us;
 // with one block a tile 519).
-struct Launch { bool wide; int tiles, nsplit; bool kwide; int ktiles, sink_tiles, nchunk; };
+struct Launch { bool wide; int tiles, nsplit; bool kwide; int ktiles, sink_tiles, nchunk; };      // sink_tiles: key tiles whose rows are dealt out
 Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right, int sinks) {
   Launch p;
   const int64_t rows = Nq > 0 ? (int64_t)Nq * group : 1, bk = (int64_t)B * kv;
@@ -930,7 +934,7 @@ Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right
   p.nsplit = 1;
   const int64_t span = left >= FAR || right >= FAR ? Nk : (int64_t)left + right + sinks + 32;
   const int64_t rounds = ((span < Nk ? span : Nk) + 127) / 128;      // 32-key tiles for each of the four waves
-  if (!p.wide && p.tiles * bk < 256) {
+  if (!p.wide && p.tiles * bk < 256 && rounds >= 16 + rows * bk / 512) {
     int64_t n = 512 / (p.tiles * bk);
     if (n > rounds / 4) n = rounds / 4;
     p.nsplit = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
@@ -939,14 +943,18 @@ Launch plan(int B, int kv, int group, int Nq, int Nk, int d, int left, int right
   const int kb = p.kwide ? 128 : 32;
   p.ktiles = (Nk + kb - 1) / kb;
   p.sink_tiles = 0; p.nchunk = 1;
-  if (sinks > 0 && left < FAR && Nk > 0) {
-    const int64_t usual = ((int64_t)left + (right >= FAR ? Nk : right) + kb) * group;      // rows of any other tile
-    int64_t n = rows / (usual < 128 ? 128 : usual);
-    const int64_t st = ((sinks < Nk ? sinks : Nk) + kb - 1) / kb, most = (64ll << 20) / (bk * st * 2 * kb * d);      // (256 MB of partial sums at most)
-    if (n > most) n = most;
-    p.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-    if (p.nchunk > 1) p.sink_tiles = (int)st;
-  }
+  if (Nk < 1) return p;
+  const int64_t usual = left >= FAR || right >= FAR ? rows : ((int64_t)left + right + kb) * group;      // rows of a tile without sinks
+  const int64_t seen = usual < rows ? usual : rows, tall = sinks > 0 && left < FAR ? rows / (usual < 128 ? 128 : usual) : 1, blocks = p.ktiles * bk;
+  int64_t n = blocks < 256 ? 512 / blocks : 1;
+  if (n > seen / 512) n = seen / 512;      // (four tiles of 32 rows for each of a block's four waves)
+  int64_t st = p.ktiles;
+  if (n > 1) { if (n < tall) n = tall < 8 ? tall : 8 > n ? 8 : n; }
+  else { n = tall; st = ((sinks < Nk ? sinks : Nk) + kb - 1) / kb; }
+  const int64_t most = (64ll << 20) / (bk * (st < 1 ? 1 : st) * 2 * kb * d);      // (256 MB of partial sums at most)
+  if (n > most) n = most;
+  p.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  if (p.nchunk > 1) p.sink_tiles = (int)st;
   return p;
 }
 

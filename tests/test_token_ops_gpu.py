@@ -148,6 +148,9 @@ WIN = {
     "wide_64": (2, 1100, 1100, 16, 16, 64, 150, 77, 3, 0, (1100, 900)),
     "wide_128": (1, 1033, 1033, 32, 32, 128, 200, 0, 70, 0, None),
     "wide_96_shared": (4, 700, 700, 36, 12, 96, 64, 64, 0, 0, (700, 650, 699, 1)),
+    "few_key_tiles": (1, 600, 600, 6, 2, 64, None, 0, 0, 0, None),
+    "few_key_tiles_sinks": (2, 700, 700, 6, 1, 96, 300, 40, 50, 0, (700, 333)),
+    "few_key_tiles_outside": (1, 1500, 1300, 3, 1, 128, 500, None, 40, -100, (1250,)),
     "wide_32": (8, 260, 260, 16, 16, 32, None, 0, 0, 0, None),
 }
 
