@@ -351,7 +351,7 @@ template <typename S, typename TILE, typename LAND, typename WORK>
 __device__ __forceinline__ void stream_tiles(int t0, int t1, TILE tile, LAND land, WORK work) {
   int t = t0;
   if constexpr (S::NBUF == 2) {
-    auto turn = [&](auto i) {
+    auto turn = [&](auto i) __attribute__((always_inline)) {
       loads_done();
       land(i);
       lds_barrier();
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256, (waves_fwd<T, D, WIDE>())) void k_win_fwd(cons
   const Frags<T, D> F(lane, own);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
-  auto step = [&](const char* ks, const char* vs, int u, int k0) {      // 32 keys, k0 the first of them, rows 32 u .. of the tile
+  auto step = [&](const char* ks, const char* vs, int u, int k0) __attribute__((always_inline)) {      // 32 keys, k0 the first of them, rows 32 u .. of the tile
     if (wave.none(a, k0)) return;
     v16f s = zero16();
     {
@@ -612,7 +612,7 @@ __global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArg
   const Frags<T, D> F(lane, own);
   auto key_of = [&](int t) { return (t < pl.nsink ? t : pl.w0 + t - pl.nsink) * S::KT; };
 
-  auto step = [&](const char* ks, const char* vs, int u, int k0) {
+  auto step = [&](const char* ks, const char* vs, int u, int k0) __attribute__((always_inline)) {
     if (wave.none(a, k0)) return;
     v16f s = zero16(), dp = zero16();
     two_products<T, D, read_group<T, D>()>(F, ks, vs, 32 * u, qf, [&](int k) { return gf[k]; }, s, dp);
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(256, (waves_kv<T, D>())) void k_win_dkv(const WinAr
   const int per_head = (block.hi - block.lo + S::RT - 1) / S::RT, ntile = per_head * a.group;
   const int per = shared_rows ? (ntile + a.nchunk - 1) / a.nchunk : ntile, t0 = chunk * per, t1 = min(ntile, t0 + per);
 
-  auto step = [&](const char* qs, const char* gs, const float* sl, const float* sd, int u, int i0) {      // 32 query rows, i0 the first token
+  auto step = [&](const char* qs, const char* gs, const float* sl, const float* sd, int u, int i0) __attribute__((always_inline)) {      // 32 query rows, i0 the first token
     if (i0 >= any_hi || i0 + 32 <= any_lo) return;
     v16f s = zero16(), dp = zero16();
     if constexpr (S::VLDS) two_products<T, D, 2>(F, qs, gs, 32 * u, kf, [&](int k) { return FV.rows(smem + S::vals, 0, k); }, s, dp);
