@@ -2427,7 +2427,7 @@ class RotaryAxes(torch.autograd.Function):
     def forward(ctx, x, heads, positions, rot):
         xs, (xb, xt) = _strided(x)
         B, N, W = x.shape
-        y = torch.empty((B, N, W), dtype=x.dtype, device=x.device)
+        y = x.new_empty((B, N, W))
         with _device_of(x):
             _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, 0, W // heads, 0, 0, 0, 0, 0.0, _p(positions), *rot, 0,
                       _dt(x), _stream())
@@ -2440,7 +2440,7 @@ class RotaryAxes(torch.autograd.Function):
         (positions,) = ctx.saved_tensors
         gs, (gb, gt) = _strided(g)
         B, N, W = g.shape
-        gx = torch.empty((B, N, W), dtype=g.dtype, device=g.device)
+        gx = g.new_empty((B, N, W))
         with _device_of(g):
             _lib.call("dp_qk_rotary_fwd", _p(gs), gb, gt, _p(gx), N * W, W, B, N, ctx.heads, 0, W // ctx.heads, 0, 0, 0, 0, 0.0, _p(positions),
                       *ctx.rot, 1, _dt(g), _stream())
@@ -2468,7 +2468,7 @@ class QkNormRotary(torch.autograd.Function):
         B, N, W = x.shape
         d = W // (heads + kv)
         qwd, qbd, kwd, kbd = _dense(qw, qb, kw, kb)
-        y = torch.empty((B, N, W), dtype=x.dtype, device=x.device)
+        y = x.new_empty((B, N, W))
         with _device_of(x):
             _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, kv, d, _p(qwd), _p(qbd), _p(kwd), _p(kbd), eps,
                       _p(positions), *rot, 0, _dt(x), _stream())
@@ -2484,9 +2484,9 @@ class QkNormRotary(torch.autograd.Function):
         B, N, W = g.shape
         d = W // (heads + kv)
         qwd, kwd = _dense(qw, kw)
-        gx = torch.empty((B, N, W), dtype=g.dtype, device=g.device)
-        dw = torch.empty((4, d), dtype=torch.float32, device=g.device)
-        part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=g.device)
+        gx = g.new_empty((B, N, W))
+        dw = g.new_empty((4, d), dtype=torch.float32)
+        part = g.new_empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32)
         with _device_of(g):
             _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(gs), gb, gt, 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d, _p(qwd),
                       _p(kwd), eps, _p(positions), *rot, _dt(g), _stream())
@@ -2549,9 +2549,9 @@ class WindowAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, win, start, starts, lengths):
         (qs, qst), (ks, kst), (vs, vst) = _strided(q, True), _strided(k, True), _strided(v, True)
         (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
-        o = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
+        o = q.new_empty((B, Nq, heads, d))
         need = any(ctx.needs_input_grad[:3])
-        lse = torch.empty((B * heads * Nq,), dtype=torch.float32, device=q.device) if need else None
+        lse = q.new_empty((B * heads * Nq,), dtype=torch.float32) if need else None
         with _device_of(q):
             ws = _window_ws(B, heads, kv, Nq, Nk, d, win, 0, q.device)
             _lib.call("dp_window_attention_fwd", _p(qs), *qst, _p(ks), *kst, _p(vs), *vst, _p(o), Nq * heads * d, heads * d, d, _p(lse), _p(ws),
@@ -2567,8 +2567,8 @@ class WindowAttention(torch.autograd.Function):
         qst, kst, vst, win, start = ctx.opts
         gs, gst = _strided(g, True)
         (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
-        dq = torch.empty((B, Nq, heads, d), dtype=q.dtype, device=q.device)
-        dk = torch.empty((B, Nk, kv, d), dtype=q.dtype, device=q.device)
+        dq = q.new_empty((B, Nq, heads, d))
+        dk = q.new_empty((B, Nk, kv, d))
         dv = torch.empty_like(dk)
         delta = torch.empty_like(lse)
         with _device_of(q):
@@ -2629,14 +2629,14 @@ class WindowAttentionQkv(torch.autograd.Function):
         d, es, dtc = W // (heads + 2 * kv), qkv.element_size(), _dt(qkv)
         Wq, Wqk = heads * d, (heads + kv) * d
         pre = qw is not None or positions is not None
-        o = torch.empty((B, N, Wq), dtype=qkv.dtype, device=qkv.device)
+        o = qkv.new_empty((B, N, Wq))
         need = any(ctx.needs_input_grad[:5])
-        lse = torch.empty((B * heads * N,), dtype=torch.float32, device=qkv.device) if need else None
+        lse = qkv.new_empty((B * heads * N,), dtype=torch.float32) if need else None
         with _device_of(qkv):
             qk, qkb, qkt = xs, xb, xt
             if pre:
                 ws4 = _dense(qw, qb, kw, kb) if qw is not None else (None,) * 4
-                qk, qkb, qkt = torch.empty((B, N, Wqk), dtype=qkv.dtype, device=qkv.device), N * Wqk, Wqk
+                qk, qkb, qkt = qkv.new_empty((B, N, Wqk)), N * Wqk, Wqk
                 _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(qk), qkb, qkt, B, N, heads, kv, d, *(_p(w) for w in ws4), eps, _p(positions), *rot,
                           0, dtc, _stream())
             ws = _window_ws(B, heads, kv, N, N, d, win, 0, qkv.device)
@@ -2653,17 +2653,17 @@ class WindowAttentionQkv(torch.autograd.Function):
         xb, xt, heads, kv, eps, rot, win = ctx.opts
         gs, (gb, gt) = _strided(g, True)
         B, N, W = xs.shape
-        d, es, dtc, dev = W // (heads + 2 * kv), xs.element_size(), _dt(xs), xs.device
+        d, es, dtc = W // (heads + 2 * kv), xs.element_size(), _dt(xs)
         Wq, Wqk = heads * d, (heads + kv) * d
-        gx = torch.empty((B, N, W), dtype=xs.dtype, device=dev)
+        gx = xs.new_empty((B, N, W))
         delta = torch.empty_like(lse)
         dw = None
         with _device_of(xs):
-            ws = _window_ws(B, heads, kv, N, N, d, win, 1, dev)
+            ws = _window_ws(B, heads, kv, N, N, d, win, 1, xs.device)
             src, sb, stt = (xs, xb, xt) if qk is None else (qk, N * Wqk, Wqk)
             # dq, dk: into the packed gradient, or (16-bit storage, norm / rotation still to come) into a float buffer
             wide = qk is not None and xs.dtype != torch.float32
-            dst, db, dt_, des = (torch.empty((B, N, Wqk), dtype=torch.float32, device=dev), N * Wqk, Wqk, 4) if wide else (gx, N * W, W, es)
+            dst, db, dt_, des = (xs.new_empty((B, N, Wqk), dtype=torch.float32), N * Wqk, Wqk, 4) if wide else (gx, N * W, W, es)
             _lib.call("dp_window_attention_bwd", _p(src), sb, stt, d, _p(src) + Wq * es, sb, stt, d, _p(xs) + Wqk * es, xb, xt, d, _p(o), N * Wq, Wq, d,
                       _p(gs), gb, gt, d, _p(lse), _p(delta), _p(dst), db, dt_, d, _p(dst) + Wq * des, db, dt_, d, _p(gx) + Wqk * es, N * W, W, d,
                       1 if wide else 0, _p(ws), B, heads, kv, N, N, d, win[0], win[1], win[2], 0, 0, _p(lengths), win[3], dtc, _stream())
@@ -2671,8 +2671,8 @@ class WindowAttentionQkv(torch.autograd.Function):
                 part = None
                 if qw is not None:
                     qw, kw = _dense(qw, kw)
-                    dw = torch.empty((4, d), dtype=torch.float32, device=dev)
-                    part = torch.empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32, device=dev)
+                    dw = xs.new_empty((4, d), dtype=torch.float32)
+                    part = xs.new_empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32)
                 _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d,
                           _p(qw), _p(kw), eps, _p(positions), *rot, dtc, _stream())
         return (gx, *(dw.unbind(0) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
