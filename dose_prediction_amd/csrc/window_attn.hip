@@ -916,7 +916,8 @@ int raise_lds(const void* kern, size_t smem, const char* name, std::atomic<uint6
 // Which kernel, how many blocks: decided by sizes alone.
 // Wide where it gives every CU a block, narrow below (bf16, window 256 + 256, two sequences; forward / dQ / dK, dV in us, wide against narrow):
 //   heads of 128:  96 wide blocks 21 / 27 / 38 against 15 / 20 / 22;  264: 27 / 37 / 51 against 34 / 43 / 51
-//   heads of 64:  192: 15 / 18 / 22 against 16 / 20 / 22;  264: 16 / 19 / 23 against 20 / 25 / 27;  384: 20 / 25 / 29 against 26 / 32 / 36
+//   heads of 64:  192: 15 / 18 / 22 against 13 / 16 / 17;  264: 16 / 19 / 23 against 17 / 23 / 26;  384: 20 / 25 / 29 against 22 / 29 / 31
+//   (fp32 the two come within a twentieth of each other)
 // Few rows, many keys (fewer than 256 narrow blocks): the key tiles are shared out over about 512 blocks, each with four tiles a wave or more
 // (a token of 12 heads on 4 key heads, 4 sequences of up to 32 769 keys, fp16: 22.1 + 4.3 us for the merge; over 256 blocks 22.9 + 4.0, over 1024
 // 23.6 + 6.3).  Where a wave's chain is short the merge costs more than it saves, the more so the more rows there are: 2048 rows over 1024 keys
