@@ -427,6 +427,33 @@ def test_other_stream_and_captured_graph():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), i
 
 
+def test_calls_without_a_gradient():
+    """No graph where none is asked for, the same bits as with one; a leaf that asks for a gradient gets one whatever the others do."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    heads, d, N = 2, 64, 65
+    pos = grid(4, 4, 4, 1, dev)
+    x = rnd((2, N, 3 * heads * d), 120, dev, torch.bfloat16)
+    ws = [rnd((d,), 121 + i, dev, scale=0.2) + (i + 1) % 2 for i in range(4)]
+    q, k, v = x.unflatten(-1, (3 * heads, d)).split(heads, 2)
+    rot = dict(positions=pos, sections=(12, 10, 10))
+    calls = [(lambda: ops.rotary_axes(x, 3 * heads, **rot), [x]), (lambda: ops.qk_norm_rotary(x, heads, 2 * heads, *ws, **rot), [x, *ws]),
+             (lambda: ops.window_attention(q, k, v, left=9), [q, k, v]), (lambda: ops.window_attention_qkv(x, heads, left=9, norm=ws, **rot), [x, *ws])]
+    for call, leaves in calls:
+        plain = call()
+        assert not plain.requires_grad
+        for leaf in leaves:
+            leaf.requires_grad_()
+            y = call()
+            assert y.requires_grad and torch.equal(y, plain)
+            (g,) = torch.autograd.grad(y.float().square().sum(), leaf)
+            assert g.shape == leaf.shape and torch.isfinite(g).all()
+            with torch.no_grad():
+                z = call()
+            assert not z.requires_grad and torch.equal(z, plain)
+            leaf.requires_grad_(False)
+
+
 def test_refused_on_the_gpu():
     from dose_prediction_amd import ops, _lib
     dev = _dev()
