@@ -34,6 +34,7 @@ struct QkArgs {
   int64_t xb, xt, gb, gt, yb, yt;    // element strides of sequence and token
   const float *wq, *bq, *wk, *bk;
   float* part;
+  const int* lens;                   // backward: valid tokens of every sequence (NULL: all); what lies behind has no gradient, whatever it holds
   float eps, sgn;
   int hq, hk, tok;
   int64_t N, tokens;
@@ -224,6 +225,12 @@ __global__ void __launch_bounds__(256) k_qk_rotary_bwd(const QkArgs a, const Rot
         int64_t b, r;
         locate(a.N, b0, r0, t, b, r);
         float g[16], v[16];
+        if (a.lens && r >= a.lens[b]) {      // (a head's lanes together.  Padding enters no product: 0 * NaN, or 0 * rstd of a row of zeros, is no zero)
+#pragma unroll
+          for (int e = 0; e < 16; e++) g[e] = 0.f;
+          if (on) O::store((T*)a.y + b * a.yb + r * a.yt + h * D, c, g);
+          continue;
+        }
         if (on) {
           O::load((const G*)a.g + b * a.gb + r * a.gt + h * D, c, g);
           if (NORM) O::load((const T*)a.x + b * a.xb + r * a.xt + h * D, c, v);
@@ -370,7 +377,7 @@ extern "C" int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, 
   if (!x || !y) DP_FAIL("qk_rotary_fwd: x or y missing");
   const int tok = block_tokens(tokens);
   if ((tokens + tok - 1) / tok > 0x7fffffff || (int64_t)tok * (heads + kv_heads) > 0x3fffffff) DP_FAIL("qk_rotary_fwd: too many rows");
-  QkArgs a{x, nullptr, y, xb, xt, 0, 0, yb, yt, wq, bq, wk, bk, nullptr, eps, inverse ? -1.f : 1.f, heads, kv_heads, tok, N, tokens};
+  QkArgs a{x, nullptr, y, xb, xt, 0, 0, yb, yt, wq, bq, wk, bk, nullptr, nullptr, eps, inverse ? -1.f : 1.f, heads, kv_heads, tok, N, tokens};
   const size_t smem = R.pairs ? (size_t)tok * (d / 2) * sizeof(float2) : 0;
   const dim3 grid((unsigned)((tokens + tok - 1) / tok));
   DP_DISPATCH(dtype, QK_DIMS(d, QK_IN(R.interleaved, if (norm) hipLaunchKernelGGL((k_qk_rotary_fwd<T, D, true, IN>), grid, dim3(256), smem, STREAM, a, R);
@@ -378,10 +385,10 @@ extern "C" int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, 
   DP_CHECK_LAUNCH("qk_rotary_fwd"); return 0;
 }
 
-extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const void* g, int64_t gb, int64_t gt, int g_f32, void* gx, int64_t gxb, int64_t gxt,
-                                float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
-                                const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
-                                int dtype, void* stream) {
+extern "C" int dp_qk_rotary_bwd_ragged(const void* x, int64_t xb, int64_t xt, const void* g, int64_t gb, int64_t gt, int g_f32, void* gx, int64_t gxb, int64_t gxt,
+                                       float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
+                                       const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
+                                       const int32_t* lengths, int dtype, void* stream) {
   if (B < 0 || N < 0 || heads < 0 || kv_heads < 0) DP_FAIL("qk_rotary_bwd: bad sizes B=%d N=%lld heads=%d + %d", B, (long long)N, heads, kv_heads);
   if (d != 32 && d != 64 && d != 96 && d != 128) DP_FAIL("qk_rotary_bwd: head dim %d not in {32, 64, 96, 128}", d);
   if (dtype != DP_F32 && dtype != DP_BF16 && dtype != DP_F16) DP_FAIL("qk_rotary_bwd: bad dtype %d", dtype);
@@ -401,7 +408,7 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
   if (!g || !gx) DP_FAIL("qk_rotary_bwd: g or gx missing");
   const int tok = block_tokens(tokens);
   if ((tokens + tok - 1) / tok > 0x7fffffff || (int64_t)tok * (heads + kv_heads) > 0x3fffffff) DP_FAIL("qk_rotary_bwd: too many rows");
-  QkArgs a{x, g, gx, xb, xt, gb, gt, gxb, gxt, wq, nullptr, wk, nullptr, part, eps, 1.f, heads, kv_heads, tok, N, tokens};
+  QkArgs a{x, g, gx, xb, xt, gb, gt, gxb, gxt, wq, nullptr, wk, nullptr, part, lengths, eps, 1.f, heads, kv_heads, tok, N, tokens};
   const size_t smem = R.pairs ? (size_t)tok * (d / 2) * sizeof(float2) : 0;
   const int nblk = norm ? dp_qk_rotary_parts(tokens) : (int)((tokens + tok - 1) / tok);
 #define QK_BWD(TG) DP_DISPATCH(dtype, QK_DIMS(d, QK_IN(R.interleaved, \
@@ -411,4 +418,12 @@ extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const voi
   DP_CHECK_LAUNCH("qk_rotary_bwd");
   if (norm) { hipLaunchKernelGGL(k_qk_dw_sum, dim3(cdiv(4 * d, 32)), dim3(1024), 0, STREAM, (const float*)part, dw, nblk, 4 * d); DP_CHECK_LAUNCH("qk_rotary_bwd(dw)"); }
   return 0;
+}
+
+extern "C" int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const void* g, int64_t gb, int64_t gt, int g_f32, void* gx, int64_t gxb, int64_t gxt,
+                                float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
+                                const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
+                                int dtype, void* stream) {
+  return dp_qk_rotary_bwd_ragged(x, xb, xt, g, gb, gt, g_f32, gx, gxb, gxt, part, dw, B, N, heads, kv_heads, d, wq, wk, eps, pos, pos_kind, posb, naxes, s0, s1,
+                                 s2, s3, base, interleaved, nullptr, dtype, stream);
 }

@@ -2695,8 +2695,8 @@ class WindowAttentionQkv(torch.autograd.Function):
                     qw, kw = _dense(qw, kw)
                     dw = xs.new_empty((4, d), dtype=torch.float32)
                     part = xs.new_empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32)
-                _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d,
-                          _p(qw), _p(kw), eps, _p(positions), *rot, dtc, _stream())
+                _lib.call("dp_qk_rotary_bwd_ragged", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads,
+                          kv, d, _p(qw), _p(kw), eps, _p(positions), *rot, _p(lengths), dtc, _stream())
         return (gx, *(dw.unbind(0) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
 
 
@@ -2704,7 +2704,8 @@ def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks
                          positions=None, sections=None, base=10000.0, interleaved=False):
     """The attention block's core on the packed projection [B, N, (heads + 2 kv_heads) * d] ("q heads | k heads | v heads", kv_heads None:
     as many as heads), as attention() takes it: with norm = (q_weight, q_bias, k_weight, k_bias) the LayerNorm of qk_norm_rotary, with
-    positions the rotation of rotary_axes, then window_attention of the rows with themselves.  Returns [B, N, heads * d]."""
+    positions the rotation of rotary_axes, then window_attention of the rows with themselves.  Returns [B, N, heads * d].  Rows outside
+    [0, lengths[b]) add nothing to the norm's gradients either, whatever they and their positions hold."""
     what = "window_attention_qkv"
     norm = tuple(norm) if norm is not None else (None,) * 4
     if len(norm) != 4:

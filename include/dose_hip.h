@@ -217,7 +217,9 @@ int dp_add_layernorm_bwd_det(const void* x, const void* gy, const void* gsum, co
  *   inverse != 0 turns back (the gradient of the rotation alone).  y may be x.
  * dp_qk_rotary_bwd: gx from gy (g_f32 != 0: gy is float whatever the storage type; gx may be gy where the types agree); with a norm also
  * dw[4][d] = gradients of wq, bq, wk, bk (OVERWRITTEN; those of a group without heads are zero), from part, a scratch of
- * dp_qk_rotary_parts(B * N) x 4 x d floats, added in a fixed order.  Without a norm x, part and dw may be NULL. */
+ * dp_qk_rotary_parts(B * N) x 4 x d floats, added in a fixed order.  Without a norm x, part and dw may be NULL.
+ * dp_qk_rotary_bwd_ragged: sequence b is lengths[b] tokens long (device int32; <= 0: empty, past N: all N; NULL: all).  Tokens behind it get
+ * gx = 0 and add nothing to dw, whatever x, g and pos hold there. */
 int dp_qk_rotary_parts(int64_t tokens);
 int dp_qk_rotary_fwd(const void* x, int64_t xb, int64_t xt, void* y, int64_t yb, int64_t yt, int B, int64_t N, int heads, int kv_heads, int d,
                      const float* wq, const float* bq, const float* wk, const float* bk, float eps, const void* pos, int pos_kind, int64_t posb,
@@ -226,6 +228,10 @@ int dp_qk_rotary_bwd(const void* x, int64_t xb, int64_t xt, const void* g, int64
                      float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
                      const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
                      int dtype, void* stream);
+int dp_qk_rotary_bwd_ragged(const void* x, int64_t xb, int64_t xt, const void* g, int64_t gb, int64_t gt, int g_f32, void* gx, int64_t gxb, int64_t gxt,
+                            float* part, float* dw, int B, int64_t N, int heads, int kv_heads, int d, const float* wq, const float* wk, float eps,
+                            const void* pos, int pos_kind, int64_t posb, int naxes, int s0, int s1, int s2, int s3, double base, int interleaved,
+                            const int32_t* lengths, int dtype, void* stream);
 
 /* ---- attention over a sliding window whose first tokens stay visible (beside dp_attention_*, for token rows too long for it) ------------
  * q, o, go, dq: [B][Nq][heads][d], k, v, dk, dv: [B][Nk][kv_heads][d], each with its own element strides of sequence, token and head (rows

@@ -1,0 +1,77 @@
+"""Token operators on the GPU: what their documentation promises of calls at its edges -- padding behind the norm and the rotation, tensors whose
+outer strides mean nothing, recorded programs, gradients of gradients, the wide kernels behind the packed projection."""
+import math
+
+import pytest
+import torch
+
+from oracle import ref_tokens as R
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda:0")
+
+
+def rnd(shape, seed, dev, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dev, dtype)
+
+
+def norms(d, seed, dev):
+    return [(rnd((d,), seed + i, dev, scale=0.2) + (i + 1) % 2).requires_grad_() for i in range(4)]
+
+
+# ------------------------------------------------------------------------------------------------ padding of a packed projection
+# (heads, kv, d, interleaved, norm, rotary)
+PACKED = [(4, 4, 64, False, True, True), (6, 2, 128, True, True, False), (4, 2, 96, True, False, True), (3, 3, 32, False, True, True)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", PACKED)
+def test_packed_padding_may_hold_anything(dtype, case):
+    """Rows outside the sequences -- the projection, the incoming gradient, the positions -- hold NaN or infinities: the same bits everywhere
+    else, the norm's gradients among them, and zeros for their own gradient.  One sequence is empty, one is longer than the rows."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    heads, kv, d, inter, norm, rot = case
+    B, N = 4, 67
+    lengths = torch.tensor([N, 0, 30, N + 5], dtype=torch.int32, device=dev)
+    pad = torch.arange(N, device=dev) >= lengths[:, None]
+    pos = torch.randint(0, 900, (B, N, 3), generator=torch.Generator().manual_seed(1)).to(dev, torch.float32)
+    x, g = rnd((B, N, (heads + 2 * kv) * d), 2, dev, dtype), rnd((B, N, heads * d), 3, dev, dtype)
+    ws = norms(d, 4, dev) if norm else []
+
+    def step(x, g, pos):
+        x = x.clone().requires_grad_()
+        extra = dict(positions=pos, sections=(d // 2 - 2 * (d // 6), d // 6, d // 6), interleaved=inter) if rot else {}
+        y = ops.window_attention_qkv(x, heads, kv, left=20, right=13, sinks=2, lengths=lengths, norm=ws or None, **extra)
+        return (y.detach(), *torch.autograd.grad(y, [x, *ws], g))
+    want = step(x, g, pos)
+    for t in want:
+        assert torch.isfinite(t).all()
+    assert not want[0][pad].any() and not want[1][pad].any()
+    for bad in (math.nan, math.inf, -math.inf):
+        got = step(*(t.masked_fill(pad[..., None], bad) for t in (x, g, pos)))
+        for name, a, b in zip(("out", "dqkv", "q_weight", "q_bias", "k_weight", "k_bias"), got, want):
+            assert torch.equal(a, b), (name, bad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_packed_padding_of_zeros_without_eps(dtype):
+    """eps = 0 and a zero row behind the sequence: its variance is zero, its gradients are still none."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    heads, d, N = 2, 64, 40
+    lengths = torch.tensor([25, 40], dtype=torch.int32, device=dev)
+    x = rnd((2, N, 3 * heads * d), 10, dev, dtype)
+    x[0, 25:] = 0
+    x.requires_grad_()
+    ws = norms(d, 11, dev)
+    y = ops.window_attention_qkv(x, heads, left=9, norm=ws, eps=0.0, lengths=lengths)
+    grads = torch.autograd.grad(y, [x, *ws], rnd((2, N, heads * d), 15, dev, dtype))
+    assert all(torch.isfinite(t).all() for t in (y, *grads)) and not grads[0][0, 25:].any()
+    assert all(t.any() for t in grads)
