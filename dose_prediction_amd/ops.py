@@ -2365,8 +2365,10 @@ class _NoContext:
 
 
 def _run(fn, leaves, *args):
-    """fn.apply(*leaves, *args), without a node of the graph where none of the leaves asks for a gradient (a call: 11.9 us of host time instead of 15.6)."""
-    if getattr(_fwd_ad, "_current_level", -1) < 0:      # (forward-mode derivatives are refused by apply)
+    """fn.apply(*leaves, *args), without a node of the graph where none of the leaves asks for a gradient (a call: 11.9 us of host time instead of 15.6).
+    A recording (torch.jit.trace) holds the node or nothing of the call, and forward-mode derivatives are refused by it: both always get it (also where
+    torch does not say whether a forward-mode level is open)."""
+    if getattr(_fwd_ad, "_current_level", 0) < 0 and not torch.jit.is_tracing():
         if not torch.is_grad_enabled():
             return fn.forward(_NoContext(), *leaves, *args)
         for t in leaves:
@@ -2391,6 +2393,8 @@ def _strided(t, tiles=False):
     return t, t.stride()[:-1]
 
 
+# (The functions check their arguments in forward(): a recorded call comes in there again, with tensors of other sizes.  Sizes are made ints there,
+# because they are tensors while a recording runs.)
 def _head_dim(width, heads, what):
     if heads < 1 or width % heads:
         raise ValueError(f"{what}: {width} channels do not divide into {heads} heads")
@@ -2422,7 +2426,7 @@ def _rotary_args(what, x, d, positions, sections, base, interleaved):
     if sections is None:
         raise ValueError(f"{what}: positions need sections (rotated pairs of a head per axis)")
     plan = _rotary_plan(what, d, tuple(sections), base, interleaved)
-    B, N, shape, axes = x.shape[0], x.shape[1], positions.shape, plan[0]
+    (B, N), shape, axes = map(int, x.shape[:2]), tuple(map(int, positions.shape)), plan[0]
     kind = _POS_KIND.get(positions.dtype)
     if kind is None:
         raise TypeError(f"{what}: positions are int32, int64 or float32, got {positions.dtype}")
@@ -2446,12 +2450,19 @@ def _dense(*ws):
 
 class RotaryAxes(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, heads, positions, rot):
+    def forward(ctx, x, heads, positions, sections, base, interleaved):
+        what = "rotary_axes"
+        _dt(x)
+        if x.dim() != 3:
+            raise ValueError(f"{what}: x is [B, N, channels], got {tuple(x.shape)}")
+        B, N, W = map(int, x.shape)
+        d = _head_dim(W, heads, what)
+        positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
+        _chk_dev(x)
         xs, (xb, xt) = _strided(x)
-        B, N, W = x.shape
         y = x.new_empty((B, N, W))
         with _device_of(x):
-            _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, 0, W // heads, 0, 0, 0, 0, 0.0, _p(positions), *rot, 0,
+            _lib.call("dp_qk_rotary_fwd", _p(xs), xb, xt, _p(y), N * W, W, B, N, heads, 0, d, 0, 0, 0, 0, 0.0, _p(positions), *rot, 0,
                       _dt(x), _stream())
         ctx.save_for_backward(positions)
         ctx.heads, ctx.rot = heads, rot
@@ -2466,7 +2477,7 @@ class RotaryAxes(torch.autograd.Function):
         with _device_of(g):
             _lib.call("dp_qk_rotary_fwd", _p(gs), gb, gt, _p(gx), N * W, W, B, N, ctx.heads, 0, W // ctx.heads, 0, 0, 0, 0, 0.0, _p(positions),
                       *ctx.rot, 1, _dt(g), _stream())
-        return gx, None, None, None
+        return gx, None, None, None, None, None
 
 
 def rotary_axes(x, heads, positions, sections, base=10000.0, interleaved=False):
@@ -2474,21 +2485,22 @@ def rotary_axes(x, heads, positions, sections, base=10000.0, interleaved=False):
     by its token's angle.  positions [N, axes] or [B, N, axes] (int32, int64 or float32); sections: rotated pairs of a head per axis -- pair e
     of an axis with n pairs turns by position * base^(-e / n); pairs behind the sections stay.  interleaved False: pair i = channels
     (i, i + d / 2), True: (2 i, 2 i + 1).  d in HEAD_DIMS.  The gradient is the turn backwards; positions have none."""
-    _dt(x)
-    if x.dim() != 3:
-        raise ValueError(f"rotary_axes: x is [B, N, channels], got {tuple(x.shape)}")
-    d = _head_dim(x.shape[-1], heads, "rotary_axes")
-    positions, rot = _rotary_args("rotary_axes", x, d, positions, sections, base, interleaved)
-    _chk_dev(x)
-    return _run(RotaryAxes, (x,), int(heads), positions, rot)
+    return _run(RotaryAxes, (x,), int(heads), positions, sections, base, interleaved)
 
 
 class QkNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, qw, qb, kw, kb, heads, kv, eps, positions, rot):
+    def forward(ctx, x, qw, qb, kw, kb, heads, kv, eps, positions, sections, base, interleaved):
+        what = "qk_norm_rotary"
+        _dt(x)
+        if x.dim() != 3 or heads < 1 or kv < 1:
+            raise ValueError(f"{what}: x is [B, N, channels] with heads and kv_heads of at least 1, got {tuple(x.shape)}, {heads}, {kv}")
+        B, N, W = map(int, x.shape)
+        d = _head_dim(W, heads + kv, what)
+        _check_norm(what, d, qw, qb, kw, kb)
+        positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
+        _chk_dev(x, qw, qb, kw, kb)
         xs, (xb, xt) = _strided(x)
-        B, N, W = x.shape
-        d = W // (heads + kv)
         qwd, qbd, kwd, kbd = _dense(qw, qb, kw, kb)
         y = x.new_empty((B, N, W))
         with _device_of(x):
@@ -2512,7 +2524,7 @@ class QkNormRotary(torch.autograd.Function):
         with _device_of(g):
             _lib.call("dp_qk_rotary_bwd", _p(xs), xb, xt, _p(gs), gb, gt, 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads, kv, d, _p(qwd),
                       _p(kwd), eps, _p(positions), *rot, _dt(g), _stream())
-        return (gx, *dw.unbind(0), None, None, None, None, None)
+        return (gx, *dw.unbind(0), None, None, None, None, None, None, None)
 
 
 def qk_norm_rotary(x, heads, kv_heads, q_weight, q_bias, k_weight, k_bias, eps=1e-5, positions=None, sections=None, base=10000.0,
@@ -2520,15 +2532,7 @@ def qk_norm_rotary(x, heads, kv_heads, q_weight, q_bias, k_weight, k_bias, eps=1
     """LayerNorm of every head of queries and keys -- x [B, N, (heads + kv_heads) * d], rows may be slices of wider ones; one float32 [d]
     weight and bias for all query heads, one for all key heads -- and, with positions, the rotation of rotary_axes behind it, in one pass.
     The weights' gradients are added up in a fixed order."""
-    what = "qk_norm_rotary"
-    _dt(x)
-    if x.dim() != 3 or heads < 1 or kv_heads < 1:
-        raise ValueError(f"{what}: x is [B, N, channels] with heads and kv_heads of at least 1, got {tuple(x.shape)}, {heads}, {kv_heads}")
-    d = _head_dim(x.shape[-1], heads + kv_heads, what)
-    _check_norm(what, d, q_weight, q_bias, k_weight, k_bias)
-    positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
-    _chk_dev(x, q_weight, q_bias, k_weight, k_bias)
-    return _run(QkNormRotary, (x, q_weight, q_bias, k_weight, k_bias), int(heads), int(kv_heads), float(eps), positions, rot)
+    return _run(QkNormRotary, (x, q_weight, q_bias, k_weight, k_bias), int(heads), int(kv_heads), float(eps), positions, sections, base, interleaved)
 
 
 # ------------------------------------------------------------------------------------------------ attention over a sliding window
@@ -2565,12 +2569,30 @@ def _window_ws(B, heads, kv, Nq, Nk, d, win, backward, dev):
 
 
 class WindowAttention(torch.autograd.Function):
-    """q [B, Nq, heads, d], k / v [B, Nk, kv, d]; win = (left, right, sinks, scale)."""
+    """q [B, Nq, heads, d], k / v [B, Nk, kv, d]."""
 
     @staticmethod
-    def forward(ctx, q, k, v, win, start, starts, lengths):
+    def forward(ctx, q, k, v, left, right, sinks, scale, start, lengths):
+        what = "window_attention"
+        _dt(q)
+        if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+            raise ValueError(f"{what}: q [B, Nq, heads, d], k and v [B, Nk, kv_heads, d], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
+            raise TypeError(f"{what}: q, k and v share type and device, got {q.dtype}, {k.dtype}, {v.dtype} on {q.device}, {k.device}, {v.device}")
+        (B, Nq, heads, d), (Nk, kv) = map(int, q.shape), map(int, k.shape[1:3])
+        if heads < 1 or kv < 1 or heads % kv:
+            raise ValueError(f"{what}: {heads} query heads do not divide over {kv} key heads")
+        _head_dim(heads * d, heads, what)
+        win = _window_args(what, left, right, sinks, scale, d)
+        starts = None
+        if torch.is_tensor(start):
+            starts, start = _per_sequence(what, "q_start", start, B, q), 0
+        start = int(start)
+        if abs(start) >= 1 << 30:
+            raise ValueError(f"{what}: q_start {start}")
+        lengths = _per_sequence(what, "lengths", lengths, B, q)
+        _chk_dev(q)
         (qs, qst), (ks, kst), (vs, vst) = _strided(q, True), _strided(k, True), _strided(v, True)
-        (B, Nq, heads, d), (Nk, kv) = q.shape, k.shape[1:3]
         o = q.new_empty((B, Nq, heads, d))
         need = any(ctx.needs_input_grad[:3])
         lse = q.new_empty((B * heads * Nq,), dtype=torch.float32) if need else None
@@ -2598,7 +2620,7 @@ class WindowAttention(torch.autograd.Function):
             _lib.call("dp_window_attention_bwd", _p(q), *qst, _p(k), *kst, _p(v), *vst, _p(o), Nq * heads * d, heads * d, d, _p(gs), *gst, _p(lse),
                       _p(delta), _p(dq), Nq * heads * d, heads * d, d, _p(dk), Nk * kv * d, kv * d, d, _p(dv), Nk * kv * d, kv * d, d, 0, _p(ws), B,
                       heads, kv, Nq, Nk, d, win[0], win[1], win[2], start, _p(starts), _p(lengths), win[3], _dt(q), _stream())
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def window_attention(q, k, v, left=None, right=None, sinks=0, q_start=0, lengths=None, scale=None):
@@ -2610,25 +2632,7 @@ def window_attention(q, k, v, left=None, right=None, sinks=0, q_start=0, lengths
     int64 [B], None: all Nk keys): rows at positions outside [0, lengths[b]) give 0 and get and cause no gradient, whatever they hold, NaN
     included.  (A value that is not finite inside a sequence reaches the rows it is seen by, and may reach others near them.)
     scale None: d^-1/2.  Sums are added in a fixed order: the same inputs give the same bits."""
-    what = "window_attention"
-    _dt(q)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{what}: q [B, Nq, heads, d], k and v [B, Nk, kv_heads, d], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if not q.dtype == k.dtype == v.dtype or not q.device == k.device == v.device:
-        raise TypeError(f"{what}: q, k and v share type and device, got {q.dtype}, {k.dtype}, {v.dtype} on {q.device}, {k.device}, {v.device}")
-    B, heads, kv, d = q.shape[0], q.shape[2], k.shape[2], q.shape[3]
-    if heads < 1 or kv < 1 or heads % kv:
-        raise ValueError(f"{what}: {heads} query heads do not divide over {kv} key heads")
-    _head_dim(heads * d, heads, what)
-    win = _window_args(what, left, right, sinks, scale, d)
-    starts = None
-    if torch.is_tensor(q_start):
-        starts, q_start = _per_sequence(what, "q_start", q_start, B, q), 0
-    if abs(int(q_start)) >= 1 << 30:
-        raise ValueError(f"{what}: q_start {q_start}")
-    lengths = _per_sequence(what, "lengths", lengths, B, q)
-    _chk_dev(q)
-    return _run(WindowAttention, (q, k, v), win, int(q_start), starts, lengths)
+    return _run(WindowAttention, (q, k, v), left, right, sinks, scale, q_start, lengths)
 
 
 def check_attention_options(width, heads, left, right, sinks, sections, base, interleaved):
@@ -2645,10 +2649,19 @@ class WindowAttentionQkv(torch.autograd.Function):
     place; the backward pass writes one packed gradient, that of q and k passing through the norm and the rotation unrounded (float)."""
 
     @staticmethod
-    def forward(ctx, qkv, qw, qb, kw, kb, heads, kv, eps, positions, rot, win, lengths):
+    def forward(ctx, qkv, qw, qb, kw, kb, heads, kv, eps, positions, sections, base, interleaved, left, right, sinks, scale, lengths):
+        what, es, dtc = "window_attention_qkv", qkv.element_size(), _dt(qkv)
+        if qkv.dim() != 3 or heads < 1 or kv < 1 or heads % kv:
+            raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
+        B, N, W = map(int, qkv.shape)
+        d = _head_dim(W, heads + 2 * kv, what)
+        if qw is not None:
+            _check_norm(what, d, qw, qb, kw, kb)
+        positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
+        win = _window_args(what, left, right, sinks, scale, d)
+        lengths = _per_sequence(what, "lengths", lengths, B, qkv)
+        _chk_dev(qkv, qw, qb, kw, kb)
         xs, (xb, xt) = _strided(qkv, True)
-        B, N, W = qkv.shape
-        d, es, dtc = W // (heads + 2 * kv), qkv.element_size(), _dt(qkv)
         Wq, Wqk = heads * d, (heads + kv) * d
         pre = qw is not None or positions is not None
         o = qkv.new_empty((B, N, Wq))
@@ -2697,7 +2710,7 @@ class WindowAttentionQkv(torch.autograd.Function):
                     part = xs.new_empty((_lib.lib().dp_qk_rotary_parts(B * N), 4, d), dtype=torch.float32)
                 _lib.call("dp_qk_rotary_bwd_ragged", _p(xs), xb, xt, _p(dst), db, dt_, 1 if wide else 0, _p(gx), N * W, W, _p(part), _p(dw), B, N, heads,
                           kv, d, _p(qw), _p(kw), eps, _p(positions), *rot, _p(lengths), dtc, _stream())
-        return (gx, *(dw.unbind(0) if dw is not None else (None,) * 4), None, None, None, None, None, None, None)
+        return (gx, *(dw.unbind(0) if dw is not None else (None,) * 4), *(None,) * 12)
 
 
 def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks=0, lengths=None, scale=None, norm=None, eps=1e-5,
@@ -2710,18 +2723,8 @@ def window_attention_qkv(qkv, heads, kv_heads=None, left=None, right=None, sinks
     norm = tuple(norm) if norm is not None else (None,) * 4
     if len(norm) != 4:
         raise ValueError(f"{what}: norm is (q_weight, q_bias, k_weight, k_bias)")
-    _dt(qkv)
-    kv = int(heads if kv_heads is None else kv_heads)
-    if qkv.dim() != 3 or heads < 1 or kv < 1 or heads % kv:
-        raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
-    d = _head_dim(qkv.shape[-1], heads + 2 * kv, what)
-    if norm[0] is not None:
-        _check_norm(what, d, *norm)
-    positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
-    win = _window_args(what, left, right, sinks, scale, d)
-    lengths = _per_sequence(what, "lengths", lengths, qkv.shape[0], qkv)
-    _chk_dev(qkv, *norm)
-    return _run(WindowAttentionQkv, (qkv, *norm), int(heads), kv, float(eps), positions, rot, win, lengths)
+    return _run(WindowAttentionQkv, (qkv, *norm), int(heads), int(heads if kv_heads is None else kv_heads), float(eps), positions, sections, base,
+                interleaved, left, right, sinks, scale, lengths)
 
 
 # ------------------------------------------------------------------------------------------------ misc

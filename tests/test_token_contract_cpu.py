@@ -1,0 +1,82 @@
+"""Token operators without a GPU: what reaches a call of them, with the launches replaced."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The names of the entry points that a call launches; nothing is launched, any device's tensors pass."""
+    from dose_prediction_amd import ops, _lib
+    names = []
+    monkeypatch.setattr(_lib, "call", lambda name, *args: names.append(name) or 0)
+    monkeypatch.setattr(ops, "_chk_dev", lambda *ts: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_device_of", lambda t: ops._NO_GUARD)
+    return names
+
+
+def _calls(N=9, heads=2, d=64):
+    """(name, call of the packed projection)"""
+    from dose_prediction_amd import ops
+    pos = torch.zeros(N, 3, dtype=torch.int32)
+    rot = dict(positions=pos, sections=(12, 10, 10))
+    ws = [torch.ones(d) for _ in range(4)]
+
+    def parts(t):
+        return t.unflatten(-1, (3 * heads, d)).split(heads, 2)
+    return [("rotary_axes", lambda t: ops.rotary_axes(t, 3 * heads, **rot)),
+            ("qk_norm_rotary", lambda t: ops.qk_norm_rotary(t, heads, 2 * heads, *ws, **rot)),
+            ("window_attention", lambda t: ops.window_attention(*parts(t), left=3)),
+            ("window_attention_qkv", lambda t: ops.window_attention_qkv(t, heads, left=3, norm=ws, **rot))]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+def test_recorded_calls_launch_when_they_are_replayed(launches, grad):
+    for name, call in _calls():
+        x = torch.zeros(2, 9, 6 * 64, requires_grad=grad)
+        traced = torch.jit.trace(call, (x,), check_trace=False)
+        del launches[:]
+        call(x)
+        want = list(launches)
+        assert want
+        for mode in (torch.no_grad, torch.enable_grad):
+            del launches[:]
+            with mode():
+                traced(torch.ones_like(x))
+            assert launches == want, name
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recorded_calls_check_the_sizes_of_the_replay(launches):
+    """What the recording holds as constants (positions, lengths, weights) must fit the tensors that a replay brings, or nothing is launched."""
+    from dose_prediction_amd import ops
+    x, n = torch.zeros(2, 9, 6 * 64), torch.tensor([9, 3])
+    pad = ("window_attention(lengths)", lambda t: ops.window_attention(*t.unflatten(-1, (6, 64)).split(2, 2), lengths=n))
+    for name, call in [*_calls(), pad]:
+        traced = torch.jit.trace(call, (x,), check_trace=False)
+        del launches[:]
+        for other in ((2, 12, 6 * 64), (2, 9, 6 * 32), (3, 9, 6 * 64)):
+            if {"window_attention": True, pad[0]: other[0] == 2, "rotary_axes": other[1] == 9}.get(name, other == (3, 9, 6 * 64)):
+                continue      # (these fit)
+            with pytest.raises((ValueError, RuntimeError)):
+                traced(torch.zeros(other))
+            assert not launches, (name, other)
+
+
+def test_forward_derivatives_are_refused(launches, monkeypatch):
+    """Before any launch: a tangent is never dropped, whether or not torch says that a level of forward-mode derivatives is open."""
+    from dose_prediction_amd import ops
+    x = torch.zeros(2, 9, 6 * 64)
+    for known in (True, False):
+        if not known:
+            monkeypatch.setattr(ops, "_fwd_ad", object())
+        for name, call in _calls():
+            with torch.autograd.forward_ad.dual_level():
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+            for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.vjp(f, x)[1](x), lambda f: torch.func.vmap(f)(x.unsqueeze(0))):
+                del launches[:]
+                with pytest.raises(RuntimeError):
+                    transform(call)
+                assert not launches, name

@@ -75,3 +75,50 @@ def test_packed_padding_of_zeros_without_eps(dtype):
     grads = torch.autograd.grad(y, [x, *ws], rnd((2, N, heads * d), 15, dev, dtype))
     assert all(torch.isfinite(t).all() for t in (y, *grads)) and not grads[0][0, 25:].any()
     assert all(t.any() for t in grads)
+
+
+# ------------------------------------------------------------------------------------------------ recorded programs
+def _calls(dev, dtype=torch.bfloat16, N=65, heads=2, d=64):
+    """(name, call of one tensor, that tensor): every operator as a function of the packed projection."""
+    from dose_prediction_amd import ops
+    x = rnd((2, N, 3 * heads * d), 20, dev, dtype)
+    pos = torch.arange(3 * N, device=dev).reshape(N, 3)
+    ws = [w.detach() for w in norms(d, 21, dev)]
+    rot = dict(positions=pos, sections=(12, 10, 10))
+    n = torch.tensor([N, 40], device=dev)
+
+    def parts(t):
+        return t.unflatten(-1, (3 * heads, d)).split(heads, 2)
+    return [("rotary_axes", lambda t: ops.rotary_axes(t, 3 * heads, **rot), x),
+            ("qk_norm_rotary", lambda t: ops.qk_norm_rotary(t, heads, 2 * heads, *ws, **rot), x),
+            ("window_attention", lambda t: ops.window_attention(*parts(t), left=9, sinks=1, lengths=n), x),
+            ("window_attention_qkv", lambda t: ops.window_attention_qkv(t, heads, left=9, norm=ws, lengths=n, **rot), x)]
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_programs_launch_the_kernels():
+    """A recorded call computes on the inputs of the replay, where a gradient is asked for and where none is."""
+    dev = _dev()
+    for name, call, x in _calls(dev):
+        traced = torch.jit.trace(call, (x,), check_trace=False)
+        for i in range(3):
+            y = rnd(tuple(x.shape), 30 + i, dev, x.dtype)
+            want = call(y)
+            assert torch.equal(traced(y), want), (name, i)
+            with torch.no_grad():
+                assert torch.equal(traced(y), want), (name, i)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traced_transformer():
+    """A transformer with a window, normed queries and keys and rotary positions, recorded for inference."""
+    from dose_prediction_amd import blocks
+    dev = _dev()
+    torch.manual_seed(0)
+    net = blocks.TransformerBlock(128, 256, 2, attention=dict(window=7, sinks=1, qk_norm=True, rotary=(12, 10, 10))).to(dev).eval()
+    pos = torch.arange(3 * 40, device=dev, dtype=torch.int32).reshape(40, 3)
+    x = [rnd((2, 40, 128), 40 + i, dev) for i in range(3)]
+    with torch.no_grad():
+        traced = torch.jit.trace(net, (x[0], pos), check_trace=False)
+        for t in x:
+            assert torch.equal(traced(t, pos), net(t, pos))
