@@ -2384,8 +2384,8 @@ def _strided(t, tiles=False):
     its tokens, dimension 1, do not overlap and lie at most 16 MB apart), otherwise a contiguous copy."""
     st, es, shape = t.stride(), t.element_size(), t.shape
     if t.data_ptr() % 16 == 0 and (st[-1] == 1 or shape[-1] <= 1):
-        if t.is_contiguous() and st[-2] * es % 16 == 0 and t.numel():
-            return t, st[:-1]
+        if 1 not in shape[:-1] and t.is_contiguous() and st[-2] * es % 16 == 0 and t.numel():
+            return t, st[:-1]      # (the stride of a dimension of one may be anything, in a contiguous tensor too: below)
         if all(n <= 1 or s * es % 16 == 0 for n, s in zip(shape[:-1], st)) and not (
                 tiles and shape[1] > 1 and (st[1] < shape[-1] or st[1] * es > 1 << 24)):
             return t, [0 if n <= 1 else s for n, s in zip(shape[:-1], st)]

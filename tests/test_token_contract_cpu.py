@@ -80,3 +80,16 @@ def test_forward_derivatives_are_refused(launches, monkeypatch):
                 with pytest.raises(RuntimeError):
                     transform(call)
                 assert not launches, name
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_strides_of_single_dimensions_are_not_handed_on(tiles):
+    """Every stride that the kernels are given is a multiple of 16 bytes, or zero for a dimension of one; nothing is copied for it."""
+    from dose_prediction_amd import ops
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    for shape, stride in (((1, 5, 2, 64), (999, 128, 64, 1)), ((1, 1, 2, 64), (999, 77, 64, 1)), ((2, 1, 1, 64), (64, 3, 5, 1)), ((1, 5, 64), (7, 64, 1)),
+                          ((1, 1, 64), (7, 9, 1)), ((2, 5, 64), (320, 64, 1))):
+        t = base.as_strided(shape, stride)
+        assert t.is_contiguous()
+        same, st = ops._strided(t, tiles)
+        assert same is t and list(st) == [0 if n == 1 else s for n, s in zip(shape[:-1], stride)], shape

@@ -122,3 +122,35 @@ def test_traced_transformer():
         traced = torch.jit.trace(net, (x[0], pos), check_trace=False)
         for t in x:
             assert torch.equal(traced(t, pos), net(t, pos))
+
+
+# ------------------------------------------------------------------------------------------------ strides of dimensions of one
+def _odd_outer(t):
+    """The same values in a view whose dimensions of one have odd strides (its rows are where they were)."""
+    st = [s if n > 1 else 12345 + 2 * i for i, (n, s) in enumerate(zip(t.shape[:-1], t.stride()))]
+    return t.as_strided(t.shape, (*st, 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,heads", [(1, 2), (33, 1), (33, 2)])
+def test_strides_of_single_dimensions_do_not_matter(dtype, N, heads):
+    from dose_prediction_amd import ops
+    dev = _dev()
+    d = 64
+    pos = torch.arange(3 * N, device=dev).reshape(N, 3)
+    ws = norms(d, 51, dev)
+    rot = dict(positions=pos, sections=(12, 10, 10))
+    x, g = rnd((1, N, 3 * heads * d), 50, dev, dtype), rnd((1, N, heads * d), 55, dev, dtype)
+    g3 = rnd((1, N, 3 * heads * d), 56, dev, dtype)
+    q, k, v = (t.contiguous() for t in x.unflatten(-1, (3 * heads, d)).split(heads, 2))
+    g4 = g.unflatten(-1, (heads, d))
+    calls = [(lambda a: ops.rotary_axes(a, 3 * heads, **rot), (x,), g3), (lambda a: ops.qk_norm_rotary(a, heads, 2 * heads, *ws, **rot), (x,), g3),
+             (lambda a, b, c: ops.window_attention(a, b, c, left=5), (q, k, v), g4),
+             (lambda a: ops.window_attention_qkv(a, heads, left=5, norm=ws, **rot), (x,), g)]
+    for call, args, grad in calls:
+        plain = [t.clone().requires_grad_() for t in args]
+        odd = [_odd_outer(t.clone()).requires_grad_() for t in args]
+        assert all(t.is_contiguous() for t in odd) and any(s % 2 for t in odd for s in t.stride()[:-1])
+        want, got = call(*plain), call(*odd)
+        assert torch.equal(want, got)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, plain, grad), torch.autograd.grad(got, odd, _odd_outer(grad))))
