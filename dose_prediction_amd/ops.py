@@ -2379,6 +2379,32 @@ def _run(fn, leaves, *args):
     return fn.apply(*leaves, *args)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Gradients that were asked for with a graph: the same tensors, behind a node that refuses to be passed."""
+
+    @staticmethod
+    def forward(ctx, what, leaf, *grads):
+        ctx.what = what
+        return grads
+
+    @staticmethod
+    def backward(ctx, *gs):
+        raise RuntimeError(f"{ctx.what}: the second derivative is not defined (its gradients are constants to autograd)")
+
+
+def _first_order(backward):
+    """backward() of an operator whose gradients cannot be differentiated again: with create_graph=True they say so when it is tried."""
+    @functools.wraps(backward)
+    def wrapper(ctx, *gs):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *gs)
+        with torch.no_grad():
+            grads = backward(ctx, *gs)
+        behind = iter(_NoSecondDerivative.apply(backward.__qualname__.split(".")[0], torch.empty(0, requires_grad=True), *(g for g in grads if g is not None)))
+        return tuple(None if g is None else next(behind) for g in grads)
+    return wrapper
+
+
 def _strided(t, tiles=False):
     """(tensor, strides of all but the last dimension): t itself where its last dimension is dense and every row 16-byte aligned (tiles: and
     its tokens, dimension 1, do not overlap and lie at most 16 MB apart), otherwise a contiguous copy."""
@@ -2469,6 +2495,7 @@ class RotaryAxes(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         (positions,) = ctx.saved_tensors
         gs, (gb, gt) = _strided(g)
@@ -2511,6 +2538,7 @@ class QkNormRotary(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         xs, qw, kw, positions = ctx.saved_tensors
         xb, xt, heads, kv, eps, rot = ctx.opts
@@ -2606,6 +2634,7 @@ class WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         q, k, v, o, lse, starts, lengths = ctx.saved_tensors
         qst, kst, vst, win, start = ctx.opts
@@ -2683,6 +2712,7 @@ class WindowAttentionQkv(torch.autograd.Function):
         return o
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         xs, qk, o, lse, qw, kw, positions, lengths = ctx.saved_tensors
         xb, xt, heads, kv, eps, rot, win = ctx.opts

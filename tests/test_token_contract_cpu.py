@@ -93,3 +93,15 @@ def test_strides_of_single_dimensions_are_not_handed_on(tiles):
         assert t.is_contiguous()
         same, st = ops._strided(t, tiles)
         assert same is t and list(st) == [0 if n == 1 else s for n, s in zip(shape[:-1], stride)], shape
+
+
+def test_second_derivatives_are_refused_where_the_incoming_gradient_has_no_graph(launches):
+    """The gradient of a sum's argument is constant, that of its inputs is not: the refusal hangs on none of them."""
+    for name, call in _calls():
+        for loss in (lambda y: y.sum(), lambda y: y.square().sum()):
+            x = torch.zeros(2, 9, 6 * 64, requires_grad=True)
+            (gx,) = torch.autograd.grad(loss(call(x)), x, create_graph=True)
+            with pytest.raises(RuntimeError, match="second derivative"):
+                (gx.sum() + x.square().sum()).backward()
+            (gx,) = torch.autograd.grad(loss(call(x)), x)
+            assert not gx.requires_grad

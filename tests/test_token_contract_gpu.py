@@ -154,3 +154,20 @@ def test_strides_of_single_dimensions_do_not_matter(dtype, N, heads):
         want, got = call(*plain), call(*odd)
         assert torch.equal(want, got)
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, plain, grad), torch.autograd.grad(got, odd, _odd_outer(grad))))
+
+
+# ------------------------------------------------------------------------------------------------ gradients of gradients
+def test_second_derivatives_are_refused():
+    """create_graph=True gives the same first gradients; going through them again is an error, whether or not the incoming gradient itself asks
+    for one."""
+    dev = _dev()
+    for name, call, x in _calls(dev, torch.float32):
+        x = x.clone().requires_grad_()
+        (want,) = torch.autograd.grad(call(x).square().sum(), x)
+        (gx,) = torch.autograd.grad(call(x).square().sum(), x, create_graph=True)
+        assert torch.equal(gx, want), name
+        with pytest.raises(RuntimeError, match="second derivative"):
+            gx.square().sum().backward()
+        (gx,) = torch.autograd.grad(call(x).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (gx.square().sum() + x.square().sum()).backward()
