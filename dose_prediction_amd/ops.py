@@ -2465,6 +2465,8 @@ def _rotary_args(what, x, d, positions, sections, base, interleaved):
 
 def _check_norm(what, d, *ws):
     for w in ws:
+        if w is None:
+            raise ValueError(f"{what}: the norm has a weight and a bias for queries and for keys, one of them is None")
         if w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != d:
             raise ValueError(f"{what}: the norm's weights and biases are float32 [{d}], got {w.dtype} {tuple(w.shape)}")
 
@@ -2684,7 +2686,7 @@ class WindowAttentionQkv(torch.autograd.Function):
             raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
         B, N, W = map(int, qkv.shape)
         d = _head_dim(W, heads + 2 * kv, what)
-        if qw is not None:
+        if not qw is qb is kw is kb is None:
             _check_norm(what, d, qw, qb, kw, kb)
         positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
         win = _window_args(what, left, right, sinks, scale, d)

@@ -105,3 +105,16 @@ def test_second_derivatives_are_refused_where_the_incoming_gradient_has_no_graph
                 (gx.sum() + x.square().sum()).backward()
             (gx,) = torch.autograd.grad(loss(call(x)), x)
             assert not gx.requires_grad
+
+
+def test_a_norm_with_a_part_missing_is_refused():
+    from dose_prediction_amd import ops
+    x, w = torch.zeros(2, 9, 6 * 64), torch.ones(64)
+    for i in range(4):
+        for have in ([w] * 4, [None] * 4):
+            part = list(have)
+            part[i] = None if have[0] is w else w
+            with pytest.raises(ValueError, match="None"):
+                ops.window_attention_qkv(x, 2, norm=part)
+            with pytest.raises(ValueError, match="None"):
+                ops.qk_norm_rotary(x, 2, 4, *part)
