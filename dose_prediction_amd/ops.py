@@ -2463,12 +2463,14 @@ def _rotary_args(what, x, d, positions, sections, base, interleaved):
     return positions.contiguous(), (kind, N * axes if len(shape) == 3 and shape[0] == B else 0, *plan)
 
 
-def _check_norm(what, d, *ws):
+def _check_norm(what, x, d, *ws):
     for w in ws:
         if w is None:
             raise ValueError(f"{what}: the norm has a weight and a bias for queries and for keys, one of them is None")
         if w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != d:
             raise ValueError(f"{what}: the norm's weights and biases are float32 [{d}], got {w.dtype} {tuple(w.shape)}")
+        if w.device != x.device:
+            raise _lib.DoseHipError(f"{what}: the norm's weights on {w.device}, rows on {x.device}")
 
 
 def _dense(*ws):
@@ -2526,7 +2528,7 @@ class QkNormRotary(torch.autograd.Function):
             raise ValueError(f"{what}: x is [B, N, channels] with heads and kv_heads of at least 1, got {tuple(x.shape)}, {heads}, {kv}")
         B, N, W = map(int, x.shape)
         d = _head_dim(W, heads + kv, what)
-        _check_norm(what, d, qw, qb, kw, kb)
+        _check_norm(what, x, d, qw, qb, kw, kb)
         positions, rot = _rotary_args(what, x, d, positions, sections, base, interleaved)
         _chk_dev(x, qw, qb, kw, kb)
         xs, (xb, xt) = _strided(x)
@@ -2687,7 +2689,7 @@ class WindowAttentionQkv(torch.autograd.Function):
         B, N, W = map(int, qkv.shape)
         d = _head_dim(W, heads + 2 * kv, what)
         if not qw is qb is kw is kb is None:
-            _check_norm(what, d, qw, qb, kw, kb)
+            _check_norm(what, qkv, d, qw, qb, kw, kb)
         positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
         win = _window_args(what, left, right, sinks, scale, d)
         lengths = _per_sequence(what, "lengths", lengths, B, qkv)

@@ -118,3 +118,18 @@ def test_a_norm_with_a_part_missing_is_refused():
                 ops.window_attention_qkv(x, 2, norm=part)
             with pytest.raises(ValueError, match="None"):
                 ops.qk_norm_rotary(x, 2, 4, *part)
+
+
+def test_weights_on_another_device_are_refused(launches):
+    """(The kernels would read them through an address of the other device.)"""
+    from dose_prediction_amd import ops, _lib
+    x = torch.zeros(2, 9, 6 * 64)
+    for i in range(4):
+        ws = [torch.ones(64, device="meta" if j == i else "cpu") for j in range(4)]
+        for grad in (False, True):
+            y = x.clone().requires_grad_(grad)
+            with pytest.raises(_lib.DoseHipError, match="on meta"):
+                ops.window_attention_qkv(y, 2, norm=ws)
+            with pytest.raises(_lib.DoseHipError, match="on meta"):
+                ops.qk_norm_rotary(y, 2, 4, *ws)
+    assert not launches
