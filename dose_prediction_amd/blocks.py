@@ -397,6 +397,7 @@ class SABlock(nn.Module):
     window: None (all tokens), n or (left, right): a token sees that many before and behind it, None for no limit on a side;
     sinks: the first tokens stay visible to every token; qk_norm: LayerNorm of every head's queries and keys (keys q_norm.*, k_norm.*);
     rotary: rotated pairs of a head per axis of the positions that forward() is given; base, interleaved: as in ops.rotary_axes."""
+    full, rotary = True, None      # (what a block is that was pickled before there were options)
 
     def __init__(self, hidden_size, num_heads, dropout_rate=0.0, *, window=None, sinks=0, qk_norm=False, rotary=None, base=10000.0,
                  interleaved=False):
@@ -506,8 +507,9 @@ class ViT(nn.Module):
         # its result (ops.add_layer_norm): norm2 of the same block, then norm1 of the next block (the final ViT.norm after the last)
         first = self.blocks[0]
         n = ops.layer_norm(x, first.norm1.weight, first.norm1.bias, first.norm1.eps)
+        positions = getattr(self, "positions", None)      # (a network that was pickled before there were options has no such buffer)
         for i, blk in enumerate(self.blocks):
-            x, n = ops.add_layer_norm(x, blk.attn(n, self.positions), blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
+            x, n = ops.add_layer_norm(x, blk.attn(n) if positions is None else blk.attn(n, positions), blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
             nxt = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
             x, n = ops.add_layer_norm(x, blk.mlp(n), nxt.weight, nxt.bias, nxt.eps)
             hidden.append(x)

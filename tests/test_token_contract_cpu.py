@@ -133,3 +133,27 @@ def test_weights_on_another_device_are_refused(launches):
             with pytest.raises(_lib.DoseHipError, match="on meta"):
                 ops.qk_norm_rotary(y, 2, 4, *ws)
     assert not launches
+
+
+def test_networks_pickled_before_the_options_run_as_they_did(monkeypatch):
+    """A whole network that was stored without the attention's options comes back with full attention."""
+    import pickle
+    from dose_prediction_amd import blocks, ops
+    calls = []
+    for name, out in (("linear", lambda x, *a, **k: x), ("layer_norm", lambda x, *a: x), ("add_layer_norm", lambda x, y, *a: (x, y)), ("add", lambda x, y: x),
+                      ("attention", lambda x, heads: calls.append(heads) or x), ("gelu", lambda x: x), ("mlp", lambda x, *a, **k: x)):
+        if hasattr(ops, name):
+            monkeypatch.setattr(ops, name, out)
+    monkeypatch.setattr(blocks.PatchEmbeddingBlock, "forward", lambda self, x: x)
+    monkeypatch.setattr(blocks.MLPBlock, "forward", lambda self, x: x)
+    net = blocks.ViT(1, (32, 32, 32), (16, 16, 16), hidden_size=64, mlp_dim=64, num_layers=2, num_heads=2, pos_embed="perceptron")
+    del net._buffers["positions"]
+    net._non_persistent_buffers_set.discard("positions")
+    for blk in net.blocks:
+        for name in ("full", "rotary", "left", "right", "sinks", "qk_norm", "base", "interleaved"):
+            del blk.attn.__dict__[name]
+    old = pickle.loads(pickle.dumps(net))
+    x = torch.zeros(1, 8, 64)
+    n, hidden = old(x)
+    assert n is x and len(hidden) == 2 and calls == [2, 2]
+    assert old.blocks[0](x) is x and calls == [2, 2, 2]
