@@ -2415,7 +2415,7 @@ def _strided(t, tiles=False):
         if all(n <= 1 or s * es % 16 == 0 for n, s in zip(shape[:-1], st)) and not (
                 tiles and shape[1] > 1 and (st[1] < shape[-1] or st[1] * es > 1 << 24)):
             return t, [0 if n <= 1 else s for n, s in zip(shape[:-1], st)]
-    t = t.contiguous() if not t.is_contiguous() else t.clone()
+    t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride()[:-1]
 
 

@@ -93,6 +93,10 @@ def test_strides_of_single_dimensions_are_not_handed_on(tiles):
         assert t.is_contiguous()
         same, st = ops._strided(t, tiles)
         assert same is t and list(st) == [0 if n == 1 else s for n, s in zip(shape[:-1], stride)], shape
+        odd = torch.zeros(4097, dtype=torch.bfloat16)[1:].as_strided(shape, stride)      # (a row that is not aligned: copied)
+        copy, st = ops._strided(odd, tiles)
+        assert copy.data_ptr() % 16 == 0 and copy.shape == odd.shape and all(n == 1 or x % 8 == 0 for n, x in zip(shape, st)), shape
+        assert all(x % 8 == 0 for x in st), (shape, st)
 
 
 def test_second_derivatives_are_refused_where_the_incoming_gradient_has_no_graph(launches):
