@@ -171,3 +171,113 @@ def test_second_derivatives_are_refused():
         (gx,) = torch.autograd.grad(call(x).sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="second derivative"):
             (gx.square().sum() + x.square().sum()).backward()
+
+
+# ------------------------------------------------------------------------------------------------ the wide kernels behind the packed projection
+def within(got, want, bound, what, tiny):
+    got = got.double()
+    assert torch.isfinite(got).all(), what
+    worst = ((got - want).abs() / (bound + tiny)).max().item()
+    assert worst <= 1, f"{what}: {worst:.2f} of the bound"
+
+
+def _norm_back(x, w, g, eps=1e-5):
+    """(gx, operator bound) of a head's LayerNorm in float64: gx = rstd (g w - mean(g w) - h mean(g w h))."""
+    var, mean = torch.var_mean(x, -1, unbiased=False, keepdim=True)
+    r = (var + eps).rsqrt()
+    h, gw = (x - mean) * r, g * w
+    return r * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True)), (r, h)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("heads,kv,d,B,N", [(16, 16, 64, 2, 1100), (16, 16, 128, 2, 1030)])
+def test_packed_training_through_the_wide_kernels(dtype, norm, heads, kv, d, B, N):
+    """Enough rows that queries and keys both go through the kernels of 128 rows a block, with the sink's rows dealt to several blocks, in the
+    form that hands dq and dk on unrounded.  Against the formulas in float64 on the q and k that the attention sees (rounded once to the
+    storage type, as documented): dv by the bounds of the attention; dq and dk by the same bounds without their last rounding, carried through
+    the gradients of the rotation (|a| + |b| of a pair, 8 E of it) and of the norm (rstd |w| (1 + mean + |h| mean |h|) of it, and 4 d E of
+    that for its own sums), and one rounding of the result."""
+    from dose_prediction_amd import ops, _lib
+    dev = _dev()
+    group = heads // kv
+    win = dict(left=60, right=45, sinks=2)
+    assert (N * group + 127) // 128 * B * kv >= 256
+    one = _lib.lib().dp_window_attention_ws_elems(B, heads, kv, N, N, d, 60, 45, 2, 1)
+    assert one >= 2 * B * kv * 2 * 128 * d and one % (B * kv * 2 * 128 * d) == 0
+    pos, sec = torch.arange(3 * N, device=dev).reshape(N, 3), (d // 2 - 2 * (d // 6), d // 6, d // 6)
+    lengths = torch.tensor([N, N - 77], device=dev)
+    x = rnd((B, N, (heads + 2 * kv) * d), 60, dev, dtype).requires_grad_()
+    g = rnd((B, N, heads * d), 61, dev, dtype)
+    ws = norms(d, 62, dev) if norm else []
+    y = ops.window_attention_qkv(x, heads, kv, norm=ws or None, positions=pos, sections=sec, lengths=lengths, **win)
+    got = torch.autograd.grad(y, [x, *ws], g)
+    with torch.no_grad():
+        qk = x[..., :(heads + kv) * d]
+        qk = ops.qk_norm_rotary(qk, heads, kv, *ws, positions=pos, sections=sec) if norm else ops.rotary_axes(qk, heads + kv, pos, sec)
+    q, k = qk.unflatten(-1, (heads + kv, d)).split((heads, kv), 2)
+    v = x.detach()[..., (heads + kv) * d:].unflatten(-1, (kv, d))
+    g4 = g.unflatten(-1, (heads, d))
+    tiny = {torch.bfloat16: 1e-30, torch.float16: 2.0 ** -24}[dtype]
+    u = R.half_step(dtype)
+    # (a sequence at a time: float64 scores of 16 heads)
+    for b in range(B):
+        (out, eo), (dq, eq), (dk, ek), (dv, ev) = R.window(q[b:b + 1], k[b:b + 1], v[b:b + 1], g4[b:b + 1], lengths=lengths[b:b + 1], dtype=dtype, **win)
+        within(y[b:b + 1].detach().unflatten(-1, (heads, d)), out, eo, "out", tiny)
+        gx = got[0][b:b + 1].unflatten(-1, (heads + 2 * kv, d))
+        within(gx[:, :, heads + kv:], dv, ev, "dv", tiny)
+        gr, er = torch.cat((dq, dk), 2), torch.cat((eq - u * dq.abs(), ek - u * dk.abs()), 2)
+        back = R.rotary(gr, -pos.double(), sec)
+        err = R.pair_size(er) + 8 * R.E * R.pair_size(gr)
+        if norm:
+            xs = x.detach()[b:b + 1, :, :(heads + kv) * d].double().unflatten(-1, (heads + kv, d))
+            w = torch.cat((ws[0].detach().expand(heads, d), ws[2].detach().expand(kv, d))).double()
+            want, (r, h) = _norm_back(xs, w, back)
+            err = r * (err * w.abs() + (err * w.abs()).mean(-1, keepdim=True) + h.abs() * (err * w.abs() * h.abs()).mean(-1, keepdim=True))
+            gw = (back * w).abs()
+            err = err + 4 * d * R.E * r * (gw + gw.mean(-1, keepdim=True) + h.abs() * (gw * h.abs()).mean(-1, keepdim=True))
+            back = want
+        within(gx[:, :, :heads + kv], back, u * back.abs() + err, "dq, dk", tiny)
+    again = torch.autograd.grad(ops.window_attention_qkv(x, heads, kv, norm=ws or None, positions=pos, sections=sec, lengths=lengths, **win), [x, *ws], g)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,d,Nq", [(12, 4, 64, 1), (2, 2, 128, 1), (8, 1, 32, 4)])
+def test_gradients_of_few_queries_over_long_rows(dtype, heads, kv, d, Nq):
+    """The backward pass of the form for single tokens; every sequence has its own length, one of them none."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    B, Nk = 3, 5003
+    tiny = {torch.float32: 1e-30, torch.bfloat16: 1e-30, torch.float16: 2.0 ** -24}[dtype]
+    q, k, v = (rnd(s, 70 + i, dev, dtype).requires_grad_() for i, s in enumerate(((B, Nq, heads, d), (B, Nk, kv, d), (B, Nk, kv, d))))
+    g = rnd((B, Nq, heads, d), 74, dev, dtype)
+    lengths = torch.tensor([5003, 0, 2049], dtype=torch.int32, device=dev)
+    for left in (None, 700):
+        kw = dict(left=left, right=0, sinks=5)
+        out = ops.window_attention(q, k, v, q_start=lengths - Nq, lengths=lengths, **kw)
+        grads = torch.autograd.grad(out, (q, k, v), g)
+        want = R.window(q.detach(), k.detach(), v.detach(), g, start=lengths - Nq, lengths=lengths, dtype=dtype, **kw)
+        for name, a, (val, bound) in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), want):
+            within(a, val, bound, f"{name}, left={left}", tiny)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,d", [(6, 3, 64), (4, 4, 128), (8, 4, 32)])
+def test_one_token_of_many_sequences(dtype, heads, kv, d):
+    """Enough sequences that a token each fills the kernels of 128 rows a block, one row of them in use."""
+    from dose_prediction_amd import ops
+    dev = _dev()
+    B, Nk = 90, 333
+    assert B * kv >= 256
+    tiny = {torch.float32: 1e-30, torch.bfloat16: 1e-30, torch.float16: 2.0 ** -24}[dtype]
+    q, k, v = (rnd(s, 80 + i, dev, dtype).requires_grad_() for i, s in enumerate(((B, 1, heads, d), (B, Nk, kv, d), (B, Nk, kv, d))))
+    g = rnd((B, 1, heads, d), 84, dev, dtype)
+    lengths = torch.arange(B, dtype=torch.int32, device=dev) * 4 - 8
+    for left in (None, 65):
+        kw = dict(left=left, right=0, sinks=3)
+        out = ops.window_attention(q, k, v, q_start=lengths - 1, lengths=lengths, **kw)
+        grads = torch.autograd.grad(out, (q, k, v), g)
+        want = R.window(q.detach(), k.detach(), v.detach(), g, start=lengths - 1, lengths=lengths, dtype=dtype, **kw)
+        for name, a, (val, bound) in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads), want):
+            within(a, val, bound, f"{name}, left={left}", tiny)
