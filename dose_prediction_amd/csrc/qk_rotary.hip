@@ -13,8 +13,9 @@
 // tokens once into LDS and all heads of q and k share them.  Angles are formed in 64 bits (position * frequency, reduced to a fraction of a
 // turn) because a far position times a frequency has no fraction left in 32.
 // Measured: turning 27 648 bf16 rows of 12 heads of 64 (85 MB in and out) 15.6 us; with the norm, 13 801 fp32 rows of 16 heads of 64: forward
-// 21.6 us (113 MB), backward 37 + 4 us for the weights' sums (170 MB); a large copy moves 4.9 TB/s, what a kernel before left in the cache comes
-// faster.
+// 21.4 us (113 MB), backward 37 + 4 us for the weights' sums (170 MB), 27 648 bf16 rows of 12 heads of 64: 20.3 (85 MB), 39.4 + 4 (127 MB); a large
+// copy moves 4.9 TB/s, what a kernel before left in the cache comes faster.  1024 rows (12 heads of 128): 7.0 and 12.5 + 3.9 us for about 3 us of
+// bytes: the angles and a barrier stand in front of the loads, and the weights' sums are a launch of their own.
 #include "common.h"
 #include <math.h>
 

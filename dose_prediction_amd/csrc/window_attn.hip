@@ -14,11 +14,17 @@
 // the streamed tile read k-major from LDS (ds_read_b64_tr_b16).  Running maximum and sum are one register per lane, fp32.
 //
 // Roundings below 32 bits: P and dS go through the second product in the storage type (the matrix cores take nothing wider there), each off by
-// half a step of its own size; everything that is added up stays fp32.
-// Bound: the matrix cores and the exponentials beside them.  12 heads of 64, 13 825 tokens, window 577 + 576, one sink, bf16: forward 81 us,
-// dQ 102, dK / dV 136 + 5 for the sinks' sums; 6 heads of 128, window 1153 + 1152: 129, 209, 337 us.  Per 64 more keys a row the three take
-// 1.07, 1.27 and 1.27 PFLOP/s (measured over windows of 577 .. 2305 keys: what a large library product reaches is 1.22); the rest, a quarter at
-// that window, is the operands' first reading, which blocks that start together do not hide, and the tiles at the window's two edges.
+// half a step of its own size; the row sum adds the rounded P, the ones that the product takes, so that numerator and normaliser agree; delta reads
+// O as it was stored.  Everything that is added up stays fp32.  In the 2-norm, windows of 41 to 1153 keys: with its own rounding the result is off by
+// 2.0 .. 2.2e-3 in bf16 (the last rounding alone: 1.7e-3) and dQ, dK, dV by 2.4e-3, of which the rounded O inside delta is 0.2 .. 0.6e-3; fp16 an
+// eighth of each.
+// Bound, heads of 64: in the forward kernel the vector instructions beside the products, in dQ the matrix cores and the LDS alike, in dK / dV the
+// LDS (full attention over 8192 keys, shares of the time in which the unit works, forward / dQ / dK, dV: vector issue 66 / 60 / 50 %, matrix 44 / 54 / 53 %,
+// LDS 44 / 54 / 66 %).  12 heads, 13 825 tokens, window 576 + 576, one sink, bf16, chip at work: 75, 95 and 124 us + 5 for the sinks' sums, 0.64, 0.76
+// and 0.77 PFLOP/s (a large library product: 1.22); 64 keys more a row cost 1.07, 1.27 and 1.27 PFLOP/s (windows of 577 .. 2305 keys).  The rest is
+// empty slots: 1308 blocks on the 1024 (forward) and 768 slots that the CUs have for them are 1.3 and 1.7 rounds, 2.8 waves a SIMD on average of 4,
+// 2.4 of 3.  Tiles at the window's edges are 4 % more products than needed.
+// 6 heads of 128, window 1152 + 1152: 123, 197, 306 us, 0.76, 0.71, 0.61 PFLOP/s.
 #include "common.h"
 #include <atomic>
 
@@ -114,8 +120,11 @@ template <typename T, int D> struct Cfg {
 };
 
 // Tiles go from memory to LDS without passing registers (buffer_load ... lds: 64 lanes x 16 bytes to consecutive LDS addresses).  What keeps
-// the reads free of bank conflicts is the order of a row's 16-byte pieces: piece c of row r stands in place c ^ (r & SW), chosen by the
-// address each lane loads from.  Rows behind `left` are out of the descriptor's range and arrive as zeros.
+// the reads apart in the banks is the order of a row's 16-byte pieces: piece c of row r stands in place c ^ (r & SW), chosen by the
+// address each lane loads from.  Heads of 64 in 16 bits: the LDS works for as many cycles as the reads have bytes over 128, so nothing waits (8
+// cycles a matrix instruction in the forward kernel, 10 in dK / dV; the conflict counter shows half of every read of 8 or 16 bytes a lane all the
+// same).  Heads of 128, rows of 256 bytes: 12 instead of 8, the transposing reads take twice their cycles.
+// Rows behind `left` are out of the descriptor's range and arrive as zeros.
 typedef int v4i __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ v4i rsrc_of(const void* p, unsigned bytes) {
   const uint64_t u = (uint64_t)(uintptr_t)p;
@@ -217,7 +226,7 @@ template <typename T, int D> struct Frags {
 
 // Waves per SIMD that the register budget is cut for.  Two (256 registers) also keep the matrix accumulators in plain VGPRs: with more the
 // compiler puts them into AGPRs and copies them back and forth around every rescale and mask (24 instead of 9 vector instructions per
-// matrix instruction in the forward kernel).  One where two would spill.
+// matrix instruction in the forward kernel).  One where two would spill (fp32 dK / dV of 128, narrow: 22 registers spill even so, 92 bytes of scratch).
 template <typename T, int D, bool WIDE> constexpr int waves_fwd() { return sizeof(T) == 4 && D >= 96 ? 1 : sizeof(T) == 2 && D == 128 && WIDE ? 3 : 2; }
 template <typename T, int D> constexpr int waves_dq() { return sizeof(T) == 4 && D >= 96 ? 1 : 2; }
 template <typename T, int D> constexpr int waves_kv() { return sizeof(T) == 4 && D >= 64 ? 1 : sizeof(T) == 2 && D == 64 ? 3 : 2; }
@@ -601,7 +610,7 @@ __global__ __launch_bounds__(256, (waves_dq<T, D>())) void k_win_dq(const WinArg
 #pragma unroll
     for (int i = 0; i < 8; i++) dl += elem(of, i) * elem(gf[kk], i);
   }
-  dl = pair_sum(dl) * a.scale;
+  dl = pair_sum(dl) * a.scale;      // (from O as stored, half a step of it off: the forward pass keeps nothing wider)
   const float lse = row.live ? a.lse[(int64_t)bh * a.rows + row.r] : INFINITY;
   if (row.r < a.rows && h == 0 && (WIDE || wv == 0)) a.delta[(int64_t)bh * a.rows + row.r] = row.live ? dl : 0.f;
   v16f acc[C::DT];
@@ -917,11 +926,14 @@ int raise_lds(const void* kern, size_t smem, const char* name, std::atomic<uint6
 // Wide where it gives every CU a block, narrow below (bf16, window 256 + 256, two sequences; forward / dQ / dK, dV in us, wide against narrow):
 //   heads of 128:  96 wide blocks 21 / 27 / 38 against 15 / 20 / 22;  264: 27 / 37 / 51 against 34 / 43 / 51
 //   heads of 64:  192: 15 / 18 / 22 against 13 / 16 / 17;  264: 16 / 19 / 23 against 17 / 23 / 26;  384: 20 / 25 / 29 against 22 / 29 / 31
-//   (fp32 the two come within a twentieth of each other)
+//   (fp32 the two come within a twentieth of each other; heads of 32 and 96 go by the same rule, not measured on both sides.  The threshold does not
+//   know how many blocks a CU holds: 4, 3 and 3 for heads of 64.)
 // Few rows, many keys (fewer than 256 narrow blocks): the key tiles are shared out over about 512 blocks, each with four tiles a wave or more
 // (a token of 12 heads on 4 key heads, 4 sequences of up to 32 769 keys, fp16: 22.1 + 4.3 us for the merge; over 256 blocks 22.9 + 4.0, over 1024
 // 23.6 + 6.3).  Where a wave's chain is short the merge costs more than it saves, the more so the more rows there are: 2048 rows over 1024 keys
-// 10.5 us, split 7.6 + 4.4; 4096 over 2048 16.4 against 10.6 + 6.7; 5000 over 2500 (heads of 128) 26.8 against 18.2 + 7.4.
+// 10.5 us, split 7.6 + 4.4; 4096 over 2048 16.4 against 10.6 + 6.7; 5000 over 2500 (heads of 128) 26.8 against 18.2 + 7.4 (the rule rests on these).
+// Only the forward pass splits its keys: dQ of few queries over many keys runs on as many blocks as there are key heads and tiles of rows (the token
+// above, four sequences of 32 769 keys: 16 blocks, 251 us; its dK / dV 82 us, the forward pass 21 + 5).
 // Few key tiles: the rows that see one are dealt out in the same way (dK / dV of 1024 tokens, 12 heads of 64 on 4, every token before: 15.7 + 3.9
 // us; one block a tile 31.9; 8 heads of 96 on 2, 1000 tokens: 19.0 + 4.0 against 49.5).
 // Tiles that hold sinks: their rows are dealt to as many blocks as have the work of another tile (dK / dV of 13 825 tokens, heads of 64: 143 us;

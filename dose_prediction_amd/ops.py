@@ -2679,7 +2679,9 @@ def check_attention_options(width, heads, left, right, sinks, sections, base, in
 
 class WindowAttentionQkv(torch.autograd.Function):
     """The packed projection's form: norm and rotation of q and k into a buffer of their own (one launch, none without them), v read in
-    place; the backward pass writes one packed gradient, that of q and k passing through the norm and the rotation unrounded (float)."""
+    place; the backward pass writes one packed gradient, that of q and k passing through the norm and the rotation unrounded (float).
+    The buffer holds q and k in the storage type, which is what the matrix cores take: in 16 bits half a step of each behind the turn
+    (bf16, 4097 tokens: the result is off by 3.6e-3 in the 2-norm, by 2.4e-3 where q and k come rounded anyway)."""
 
     @staticmethod
     def forward(ctx, qkv, qw, qb, kw, kb, heads, kv, eps, positions, sections, base, interleaved, left, right, sinks, scale, lengths):
