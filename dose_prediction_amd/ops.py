@@ -2690,7 +2690,7 @@ class WindowAttentionQkv(torch.autograd.Function):
             raise ValueError(f"{what}: qkv is [B, N, channels] and kv_heads divides heads, got {tuple(qkv.shape)}, {heads}, {kv}")
         B, N, W = map(int, qkv.shape)
         d = _head_dim(W, heads + 2 * kv, what)
-        if not qw is qb is kw is kb is None:
+        if any(w is not None for w in (qw, qb, kw, kb)):
             _check_norm(what, qkv, d, qw, qb, kw, kb)
         positions, rot = _rotary_args(what, qkv, d, positions, sections, base, interleaved)
         win = _window_args(what, left, right, sinks, scale, d)
