@@ -191,7 +191,7 @@ def _norm_back(x, w, g, eps=1e-5):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("norm", [False, True])
-@pytest.mark.parametrize("heads,kv,d,B,N", [(16, 16, 64, 2, 1100), (16, 16, 128, 2, 1030)])
+@pytest.mark.parametrize("heads,kv,d,B,N", [(15, 15, 64, 2, 1100), (16, 16, 128, 2, 1030)])
 def test_packed_training_through_the_wide_kernels(dtype, norm, heads, kv, d, B, N):
     """Enough rows that queries and keys both go through the kernels of 128 rows a block, with the sink's rows dealt to several blocks, in the
     form that hands dq and dk on unrounded.  Against the formulas in float64 on the q and k that the attention sees (rounded once to the
